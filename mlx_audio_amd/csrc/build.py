@@ -6,6 +6,7 @@ Each .hip file is compiled to an object only when it or a header is newer.
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -13,9 +14,10 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 SOURCES = ["capi.hip", "ops.hip", "spectral_fwd.hip", "spectral_lane.hip", "spectral_wave.hip", "spectral_inv.hip", "logmel400.hip", "resample.hip", "bigfft.hip", "features.hip", "onset.hip", "griffinlim.hip", "gate.hip", "normalize.hip", "stem.hip"]
-HEADERS = ["fft_engine.h", "mia_internal.h", "w400_sweep_gen.inc", os.path.join(ROOT, "include", "mia.h")]
 LIB = os.path.join(HERE, "libmia_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-slp-vectorize", "-Wall", "-Wno-unused-function"]
+# no packed float32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results
+FLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS += os.environ.get("MIA_EXTRA_FLAGS", "").split()
 
 
@@ -30,16 +32,26 @@ def _mtime(path: str) -> float:
     return os.path.getmtime(path) if os.path.exists(path) else 0.0
 
 
+def _newest(path: str, seen: set) -> float:
+    """Time of the newest of a source file and the files it includes by quotes."""
+    path = os.path.normpath(path)
+    if path in seen or not os.path.exists(path):
+        return 0.0
+    seen.add(path)
+    with open(path) as f:
+        names = re.findall(r'^#include "([^"]+)"', f.read(), flags=re.M)
+    return max([_mtime(path)] + [_newest(os.path.join(os.path.dirname(path), n), seen) for n in names])
+
+
 def build(force: bool = False, verbose: bool = True) -> str:
     hipcc = _hipcc()
-    hdr_time = max(_mtime(h if os.path.isabs(h) else os.path.join(HERE, h)) for h in HEADERS)
     jobs = []
     objs = []
     for src in SOURCES:
         spath = os.path.join(HERE, src)
         opath = os.path.join(HERE, src.replace(".hip", ".o"))
         objs.append(opath)
-        if force or _mtime(opath) < max(_mtime(spath), hdr_time):
+        if force or _mtime(opath) < max(_newest(spath, set()), _mtime(os.path.abspath(__file__))):
             jobs.append([hipcc, *FLAGS, "-c", spath, "-o", opath])
 
     def run(cmd):
@@ -48,7 +60,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         subprocess.run(cmd, check=True)
 
     if jobs:
-        with ThreadPoolExecutor(max_workers=min(4, len(jobs))) as ex:
+        with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
             list(ex.map(run, jobs))
     if jobs or force or _mtime(LIB) < max(_mtime(o) for o in objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
