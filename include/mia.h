@@ -566,6 +566,56 @@ int mia_whisper_stem(const float* mel, int64_t clips, int64_t frames, int n_mels
                      const float* pos, void* out, int out_f16, void* workspace, size_t workspace_bytes,
                      void* stream);
 
+/* ---- the operators of the transformer blocks behind the stem ------------------------------
+ * Layer normalisation, the linear layer and attention, each with its backward pass
+ * (models/whisper/layers: the blocks that AudioEncoder.__call__ runs after the stem).  Element
+ * types: MIA_F32, MIA_F16, MIA_BF16; sums, statistics and every value between input and output
+ * are float32 (products of two-byte operands accumulate in float32 on the matrix cores); results
+ * are rounded once, to nearest even.  Strides are in elements, rows themselves contiguous;
+ * pointers need the alignment of their elements only (16-byte alignment is faster).  Results do
+ * not depend on the order in which workgroups run: two calls give the same bits. */
+#define MIA_F32 0
+#define MIA_F16 1
+#define MIA_BF16 2
+
+/* y[r] = (x[r] - mean) * rstd * weight + bias over rows of dim elements, rstd = 1 / sqrt(variance
+ * + eps).  weight, bias: device (dim), float32 or x's type (param_dtype, both alike), either may
+ * be NULL; y: (rows, dim) contiguous; mean, rstd: device float32 (rows), or both NULL. */
+int mia_layer_norm(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int dtype, const void* weight,
+                   const void* bias, int param_dtype, float eps, void* y, float* mean, float* rstd, void* stream);
+/* The gradients, from the statistics the forward call wrote: dx (rows, dim) contiguous of x's type;
+ * dweight, dbias: float32 (dim), or both NULL (then no workspace is needed). */
+size_t mia_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
+int mia_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
+                            const float* rstd, int64_t rows, int64_t dim, int dtype, const void* weight,
+                            int param_dtype, void* dx, float* dweight, float* dbias, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* y = act(x weight^T + bias) + residual: x (rows, in), weight (out, in), bias (out) of the
+ * operands' type or float32, residual (rows, out); bias, residual may be NULL.  preactivation,
+ * where not NULL, receives x weight^T + bias (what the backward pass of an activation needs).  y
+ * and preactivation: (rows, out) contiguous; neither may overlap an input.  GELU is the erf form,
+ * GELU_TANH its tanh approximation.  workspace: mia_linear_workspace_bytes bytes of device memory,
+ * 16-byte aligned (often 0). */
+#define MIA_ACT_NONE 0
+#define MIA_ACT_GELU 1
+#define MIA_ACT_GELU_TANH 2
+#define MIA_ACT_RELU 3
+size_t mia_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype);
+int mia_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
+               int bias_dtype, const void* residual, int64_t residual_stride, int activation, int64_t rows, int64_t in,
+               int64_t out, int dtype, void* y, void* preactivation, void* workspace, size_t workspace_bytes,
+               void* stream);
+/* The gradients with dz = dy act'(preactivation): dx = dz weight (rows, in), dweight = dz^T x
+ * (out, in), both contiguous of the operands' type, dbias = sum over rows of dz, float32 (out); each
+ * may be NULL.  The residual's gradient is dy itself.  dz is rounded to the operands' type for the
+ * two products (the matrix cores take no other), not for dbias. */
+size_t mia_linear_backward_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype, int activation);
+int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* weight,
+                        int64_t weight_stride, const void* preactivation, int64_t preactivation_stride, int activation,
+                        int64_t rows, int64_t in, int64_t out, int dtype, void* dx, void* dweight, float* dbias,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

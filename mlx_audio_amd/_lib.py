@@ -29,6 +29,8 @@ RS_PAD_MODES = {"constant": 0, "edge": 1, "reflect": 2, "symmetric": 3, "wrap": 
                 "line": 6, "antisymmetric": 7, "antireflect": 8}
 EPI_NONE, EPI_WHISPER, EPI_DB = 0, 1, 2
 STEM_F16, STEM_F32 = 0, 1
+F32, F16, BF16 = 0, 1, 2
+ACT_NONE, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
 
 
 class PlanDesc(ctypes.Structure):
@@ -172,6 +174,19 @@ SIGNATURES = {
     "mia_resample_fft_tables": (c_int, [c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mia_resample_fft": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p,
                                  c_void_p, c_size_t, c_void_p]),
+    "mia_layer_norm": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_float,
+                               c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mia_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "mia_layer_norm_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                        c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                        c_void_p]),
+    "mia_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
+    "mia_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_int, c_int64,
+                           c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mia_linear_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "mia_linear_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
+                                    c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_size_t, c_void_p]),
 }
 
 HAS_HIP_EXT: bool = False

@@ -1,0 +1,662 @@
+// The linear layer behind the encoder stem: y = act(x W^T + b) + residual, and its backward pass
+//   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz
+// as one matrix product kernel on the matrix cores, C[m][n] = sum_k A[n][k] B[m][k]:
+//
+//   forward   A = W  (n, k)  k contiguous      B = x  (m, k)  k contiguous
+//   dx        A = W  (k, n)  n contiguous      B = dz (m, k)  k contiguous
+//   dW        A = x  (k, n)  n contiguous      B = dz (k, m)  m contiguous
+//
+// (k is what is summed over, n the result's contiguous index.)  An operand whose k is contiguous
+// lies in LDS as rows of 64 bytes of k and a lane's 16-byte fragment is one ds_read_b128; the other
+// kind lies as rows of n (or m) and fragments are taken down the columns: ds_read_b64_tr_b16 for
+// two-byte types, four ds_read_b32 for float.  Nothing is transposed in memory.
+#pragma once
+#include "nn_common.h"
+
+namespace mia {
+namespace lin {
+using namespace nn;
+
+struct Epilogue {
+  const void* bias;      // (n) of the operands' type, or float (bias_f32), or null
+  int bias_f32;
+  int act;               // MIA_ACT_*
+  const void* residual;  // rows of residual_stride elements, or null
+  long long residual_stride;
+  void* z;               // (m, n) contiguous: the value before the activation, or null
+  void* out;             // (m, n) contiguous
+};
+
+struct Gemm {
+  const void* a;
+  const void* b;
+  long long lda, ldb;  // elements between rows in memory
+  int n, m, k;
+  int n_tiles, m_tiles;
+  int splits;          // parts of k, each with a plane of `partial`; 1: the epilogue runs at once
+  int k_per_split;     // a multiple of the k of a step
+  float* partial;      // (splits, m, n)
+  Epilogue e;
+};
+
+// 0.5 erfc(-x / sqrt 2) from erfc(z) = t (a1 + t (a2 + ... a5 t)) exp(-z^2), t = 1 / (1 + p z):
+// absolute error 1.5e-7 and no cancellation in the negative tail; `e` receives exp(-x^2 / 2).
+__device__ __forceinline__ float normal_cdf_fast(float x, float& e) {
+  const float z = __builtin_fabsf(x) * 0.70710678118654752440f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  e = __builtin_amdgcn_exp2f(-1.44269504088896340736f * z * z);
+  const float half_erfc = 0.5f * t * q * e;
+  return x < 0.0f ? half_erfc : 1.0f - half_erfc;
+}
+// Two-byte results: the polynomial's 1.5e-7 is far below their rounding.  float: the library's erfc.
+template <bool PRECISE>
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == MIA_ACT_GELU) {
+    if constexpr (PRECISE) return 0.5f * z * erfcf(-0.70710678118654752440f * z);
+    float e;
+    return z * normal_cdf_fast(z, e);
+  }
+  if (act == MIA_ACT_GELU_TANH) {  // z (1 + tanh u) / 2 = z / (1 + exp(-2 u))
+    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
+    if constexpr (PRECISE) return z / (1.0f + expf(-u2));
+    return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * u2));
+  }
+  if (act == MIA_ACT_RELU) return z < 0.0f ? 0.0f : z;  // keeps a NaN
+  return z;
+}
+template <bool PRECISE>
+__device__ __forceinline__ float derivative(float z, int act) {
+  if (act == MIA_ACT_GELU) {
+    float e, cdf;
+    if constexpr (PRECISE) {
+      cdf = 0.5f * erfcf(-0.70710678118654752440f * z);
+      e = expf(-0.5f * z * z);
+    } else {
+      cdf = normal_cdf_fast(z, e);
+    }
+    return fmaf(z * 0.39894228040143267794f, e, cdf);
+  }
+  if (act == MIA_ACT_GELU_TANH) {
+    // at +-20 the slope is 0 or 1 exactly; the limit keeps z^3 finite (and a NaN a NaN)
+    z = z > 20.0f ? 20.0f : (z < -20.0f ? -20.0f : z);
+    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
+    const float s = 1.0f / (1.0f + expf(-u2));
+    return fmaf(z * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), s);
+  }
+  if (act == MIA_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+  return 1.0f;
+}
+
+template <class T>
+__device__ __forceinline__ float bias_at(const Epilogue& e, int n) {
+  return e.bias_f32 ? static_cast<const float*>(e.bias)[n] : (float)static_cast<const T*>(e.bias)[n];
+}
+
+// COUNT consecutive results of row m from column n0 on, `left` of them inside the row.
+template <class T, int COUNT>
+__device__ __forceinline__ void finish(const Epilogue& e, long long m, int n0, int left, int n, float* v) {
+  constexpr int V = kPer16<T>;
+  constexpr bool PRECISE = sizeof(T) == 4;
+  if (e.bias) {
+    if (left >= COUNT) {
+      float b[COUNT];
+      if (e.bias_f32) {
+#pragma unroll
+        for (int j = 0; j < COUNT; j += 4) unpack<float>(load_piece(static_cast<const float*>(e.bias) + n0 + j, 4), b + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < COUNT; j += V) unpack<T>(load_piece(static_cast<const T*>(e.bias) + n0 + j, V), b + j);
+      }
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j) v[j] += b[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j)
+        if (j < left) v[j] += bias_at<T>(e, n0 + j);
+    }
+  }
+  const long long at = m * n + n0;
+  if (e.z) {
+    T* z = static_cast<T*>(e.z) + at;
+#pragma unroll
+    for (int j = 0; j < COUNT; j += V) store_piece(z + j, pack<T>(v + j), left - j);
+  }
+  if (e.act != MIA_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] = activate<PRECISE>(v[j], e.act);
+  }
+  if (e.residual) {
+    const T* r = static_cast<const T*>(e.residual) + m * e.residual_stride + n0;
+    float x[COUNT];
+#pragma unroll
+    for (int j = 0; j < COUNT; j += V) unpack<T>(load_piece(r + j, left - j), x + j);
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] += x[j];
+  }
+  T* out = static_cast<T*>(e.out) + at;
+#pragma unroll
+  for (int j = 0; j < COUNT; j += V) store_piece(out + j, pack<T>(v + j), left - j);
+}
+
+// 64 bytes that read as zero: the source of every piece that lies outside its operand.
+__device__ const u4 kZeros[4] = {};
+}  // namespace lin
+
+// Tile of BN x BM results, WN x WM waves.  An LDS stage holds 64 bytes of k of both operands.
+template <int BN_, int BM_, int WN_, int WM_, int STAGES_, int OCC_>
+struct LinTile {
+  static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, STAGES = STAGES_, OCC = OCC_;
+  static constexpr int NW = WN * WM, WG = 64 * NW;
+  static constexpr int TN = BN / WN, TM = BM / WM;  // a wave's part
+  static constexpr int RN = TN / 16, RM = TM / 16;  // ... in accumulators of 16 x 16
+  static constexpr int A_BYTES = BN * 64, B_BYTES = BM * 64, STAGE = A_BYTES + B_BYTES;
+  static constexpr int PA = BN / (16 * NW), PB = BM / (16 * NW);  // 1 KiB pieces per wave and stage
+  static constexpr int LDS = STAGES * STAGE;
+  static_assert(TN % 64 == 0 && TM % 16 == 0 && BN % (16 * NW) == 0 && BM % (16 * NW) == 0, "whole pieces");
+  static_assert(LDS <= 160 * 1024, "LDS budget");
+};
+using LinTile256 = LinTile<256, 256, 2, 4, 4, 1>;
+using LinTile128 = LinTile<128, 128, 2, 2, 4, 2>;
+using LinTile64 = LinTile<64, 64, 1, 4, 4, 4>;
+
+namespace lin {
+// One operand's tile in LDS and its fragments.  KC: k contiguous, LDS rows are `ROWS` operand rows
+// of four 16-byte pieces of k; otherwise LDS rows are the stage's k, ROWS elements each.  Piece c of
+// LDS row r sits at piece position c ^ swizzle(r), so that the lanes of one LDS read fall on
+// different banks; with LDS-DMA the same permutation is applied to the source addresses.
+template <class T, bool KC, int ROWS>
+struct Operand {
+  static constexpr int ES = (int)sizeof(T), V = 16 / ES;
+  static constexpr int KSTEP = 64 / ES;                           // k of a stage
+  static constexpr int PITCH = KC ? 64 : ROWS * ES;               // bytes of an LDS row
+  static constexpr int PIECES = PITCH / 16;                       // pieces of an LDS row
+  static __device__ __forceinline__ int swizzle(int r) {
+    if constexpr (KC) return (r ^ (r >> 2)) & 3;
+    // column reads touch rows r .. r + 3 (two-byte: of 8 groups of rows) at one column range
+    return ES == 2 ? (((r & 3) | ((r >> 1) & 4)) << 1) & (PIECES - 1) : ((r & 15) << 1) & (PIECES - 1);
+  }
+  // piece s of the stage: LDS byte s * 16; operand row / k of its first element
+  static __device__ __forceinline__ void where(int s, int& row, int& k) {
+    const int r = s / PIECES, c = (s % PIECES) ^ swizzle(r);
+    if constexpr (KC) {
+      row = r, k = c * V;
+    } else {
+      row = c * V, k = r;
+    }
+  }
+  // The 16-byte fragment of tile row `row0 + perm(lane & 15)`, k piece lane >> 4.  perm spreads the
+  // 16 rows as 16 (r >> 2) + (r & 3): with four accumulators at row0 = base + 4 t, lane group g of
+  // the result holds the 16 consecutive rows base + 16 g ...  (PERM; else rows row0 + r).
+  template <bool PERM>
+  static __device__ __forceinline__ u4 fragment(const unsigned char* tile, int row0, int lane) {
+    const int r15 = lane & 15, g = lane >> 4;
+    if constexpr (KC) {
+      const int row = row0 + (PERM ? 16 * (r15 >> 2) + (r15 & 3) : r15);
+      return *reinterpret_cast<const u4*>(tile + row * 64 + ((g ^ swizzle(row)) << 4));
+    } else if constexpr (ES == 2) {
+      const int col = row0 + (PERM ? 16 : 4) * (r15 & 3);  // this lane's quad of columns
+      const int k0 = 8 * g + (r15 >> 2);
+      const unsigned base = (unsigned)(unsigned long long)tile;
+      const int c = (col * 2) >> 4, in = (col * 2) & 15;
+      const s4 lo = lds_read_column4(base + k0 * PITCH + ((c ^ swizzle(k0)) << 4) + in);
+      const s4 hi = lds_read_column4(base + (k0 + 4) * PITCH + ((c ^ swizzle(k0 + 4)) << 4) + in);
+      union {
+        s4 h[2];
+        u4 u;
+      } x;
+      x.h[0] = lo, x.h[1] = hi;
+      return x.u;
+    } else {
+      const int col = row0 + (PERM ? 16 * (r15 >> 2) + (r15 & 3) : r15);
+      const int c = col >> 2, in = (col & 3) * 4;
+      u4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = 4 * g + j;
+        x[j] = *reinterpret_cast<const unsigned*>(tile + k * PITCH + ((c ^ swizzle(k)) << 4) + in);
+      }
+      return x;
+    }
+  }
+};
+}  // namespace lin
+
+// DMA: every 16-byte piece of both operands is aligned (bases, row strides) and lies either wholly
+// inside its operand or wholly outside; otherwise pieces go through registers, element by element
+// at the edges.
+template <class TL, class T, bool AKC, bool BKC, bool DMA>
+__global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) {
+  using namespace lin;
+  constexpr int ES = (int)sizeof(T);
+  using OA = Operand<T, AKC, TL::BN>;
+  using OB = Operand<T, BKC, TL::BM>;
+  constexpr int KSTEP = OA::KSTEP;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // Consecutive logical tiles go to one XCD (one L2).  Inside, columns of four tiles along m: the
+  // tiles in flight on an XCD share their rows of both operands.
+  const unsigned nb = gridDim.x, id = blockIdx.x;
+  const unsigned q8 = nb / 8, r8 = nb % 8, xcd = id % 8;
+  unsigned logical = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + id / 8;
+  const unsigned tiles = (unsigned)p.n_tiles * (unsigned)p.m_tiles;
+  const unsigned split = logical / tiles;
+  logical -= split * tiles;
+  constexpr unsigned GM = 4;
+  const unsigned group = logical / (GM * (unsigned)p.n_tiles);
+  const unsigned in_group = logical - group * GM * (unsigned)p.n_tiles;
+  const unsigned gm = min(GM, (unsigned)p.m_tiles - group * GM);
+  const int n0 = (int)(in_group / gm) * TL::BN;
+  const int m0 = (int)(group * GM + in_group % gm) * TL::BM;
+  const int k_begin = (int)split * p.k_per_split;
+  const int k_end = min(p.k, k_begin + p.k_per_split);
+  const int steps = (k_end - k_begin + KSTEP - 1) / KSTEP;
+
+  f4 acc[TL::RN][TL::RM];
+#pragma unroll
+  for (int i = 0; i < TL::RN; ++i)
+#pragma unroll
+    for (int j = 0; j < TL::RM; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int wn = (wv % TL::WN) * TL::TN, wm = (wv / TL::WN) * TL::TM;
+  auto compute = [&](const unsigned char* stage) {
+    u4 fa[TL::RN], fb[TL::RM];
+#pragma unroll
+    for (int j = 0; j < TL::RM; ++j) fb[j] = OB::template fragment<false>(stage + TL::A_BYTES, wm + 16 * j, lane);
+#pragma unroll
+    for (int i = 0; i < TL::RN; ++i)
+      fa[i] = OA::template fragment<true>(stage, wn + 64 * (i / 4) + 4 * (i % 4), lane);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < TL::RN; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::RM; ++j) acc[i][j] = Mma<T>::step(fa[i], fb[j], acc[i][j]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  if constexpr (DMA) {
+    // A ring of STAGES stages: while one is multiplied, the next STAGES - 1 are on their way.
+    constexpr int P = TL::PA + TL::PB, AHEAD = TL::STAGES - 1;
+    const char* src[P];
+    int at_k[P];
+    long long adv[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const bool isa = i < TL::PA;
+      const int s = (isa ? TL::PA * wv + i : TL::PB * wv + i - TL::PA) * 64 + lane;
+      int row, k;
+      if (isa) OA::where(s, row, k);
+      else OB::where(s, row, k);
+      row += isa ? n0 : m0;
+      const bool in = row < (isa ? p.n : p.m);
+      k += k_begin;
+      const bool kc = isa ? AKC : BKC;
+      const long long ld = isa ? p.lda : p.ldb;
+      src[i] = static_cast<const char*>(isa ? p.a : p.b) + (kc ? row * ld + k : k * ld + row) * ES;
+      adv[i] = (kc ? (long long)KSTEP : KSTEP * ld) * ES;
+      at_k[i] = in ? k : p.k;  // a row outside never comes in
+    }
+    const unsigned lds0 = (unsigned)(unsigned long long)(smem);
+    auto issue = [&](int step) {
+      const unsigned buf = lds0 + (unsigned)(step % TL::STAGES) * TL::STAGE;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const unsigned dst = buf + (i < TL::PA ? (unsigned)(TL::PA * wv + i) * 1024u
+                                               : TL::A_BYTES + (unsigned)(TL::PB * wv + i - TL::PA) * 1024u);
+        const char* from = at_k[i] < k_end ? src[i] : reinterpret_cast<const char*>(kZeros);
+        dma16(from, (unsigned)__builtin_amdgcn_readfirstlane((int)dst));
+        src[i] += adv[i];
+        at_k[i] += KSTEP;
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) issue(s);
+    for (int s = 0; s < steps; ++s) {
+      // stage s has landed for this wave; the barrier makes that all waves, and no wave still reads
+      // the stage that the next loads go to
+      wait_loads<P*(AHEAD - 1)>();
+      barrier_keep_loads();
+      issue(s + AHEAD);  // (past the end: zeros, so that the count of loads in flight stays the same)
+      compute(smem + (s % TL::STAGES) * TL::STAGE);
+    }
+    wait_loads<0>();
+  } else {
+    constexpr int P = TL::PA + TL::PB;
+    u4 held[P];
+    auto fetch = [&](int step) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const bool isa = i < TL::PA;
+        const int s = (isa ? TL::PA * wv + i : TL::PB * wv + i - TL::PA) * 64 + lane;
+        int row, k;
+        if (isa) OA::where(s, row, k);
+        else OB::where(s, row, k);
+        row += isa ? n0 : m0;
+        k += k_begin + step * KSTEP;
+        const int rows = isa ? p.n : p.m;
+        const long long ld = isa ? p.lda : p.ldb;
+        const T* base = static_cast<const T*>(isa ? p.a : p.b);
+        const bool kc = isa ? AKC : BKC;
+        held[i] = u4{0, 0, 0, 0};
+        if (kc) {
+          if (row < rows && k < k_end) held[i] = load_piece(base + row * ld + k, k_end - k);
+        } else {
+          if (row < rows && k < k_end) held[i] = load_piece(base + k * ld + row, rows - row);
+        }
+      }
+    };
+    fetch(0);
+    for (int s = 0; s < steps; ++s) {
+      unsigned char* stage = smem + (s & 1) * TL::STAGE;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const bool isa = i < TL::PA;
+        const int at = (isa ? TL::PA * wv + i : TL::PB * wv + i - TL::PA) * 1024 + lane * 16 + (isa ? 0 : TL::A_BYTES);
+        *reinterpret_cast<u4*>(stage + at) = held[i];
+      }
+      __syncthreads();  // this stage is written; every wave is done with the other one
+      if (s + 1 < steps) fetch(s + 1);
+      compute(stage);
+    }
+  }
+
+  // acc[i][j][v]: column n0 + wn + 64 (i / 4) + 16 g + 4 (i % 4) + v of row m0 + wm + 16 j + (lane & 15)
+  const int g = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < TL::RM; ++j) {
+    const long long m = m0 + wm + 16 * j + (lane & 15);
+    if (m >= p.m) continue;
+#pragma unroll
+    for (int i = 0; i < TL::RN; i += 4) {
+      const int n = n0 + wn + 16 * i + 16 * g;
+      const int left = p.n - n;
+      if (left <= 0) continue;
+      float v[16];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) v[t] = acc[i + t / 4][j][t % 4];
+      if (p.splits > 1) {
+        float* out = p.partial + ((long long)split * p.m + m) * p.n + n;
+#pragma unroll
+        for (int t = 0; t < 16; t += 4) store_piece(out + t, pack<float>(v + t), left - t);
+      } else {
+        finish<T, 16>(p.e, m, n, left, p.n, v);
+      }
+    }
+  }
+}
+
+// The parts of a product that was split along k, added in order, and the epilogue.
+template <class T>
+__global__ __launch_bounds__(256) void lin_join_kernel(lin::Gemm p) {
+  using namespace lin;
+  const int per_row = (p.n + 7) / 8;
+  const long long total = (long long)p.m * per_row;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long m = i / per_row;
+    const int n = (int)(i - m * per_row) * 8;
+    const int left = p.n - n;
+    float v[8] = {};
+    for (int s = 0; s < p.splits; ++s) {
+      const float* src = p.partial + ((long long)s * p.m + m) * p.n + n;
+      float x[8];
+      unpack<float>(load_piece(src, left), x);
+      unpack<float>(load_piece(src + 4, left - 4), x + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += x[j];
+    }
+    finish<T, 8>(p.e, m, n, left, p.n, v);
+  }
+}
+
+// Few rows of x (MT groups of 16): a stream through the weights.  A workgroup owns 16 columns of
+// the result, its waves take 64-byte steps of k in turn and their sums meet in LDS.  Fragments come
+// straight from memory: 16 bytes a lane, 64 bytes of each of 16 weight rows per load.
+template <class T, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void lin_few_kernel(lin::Gemm p) {
+  using namespace lin;
+  constexpr int ES = (int)sizeof(T), V = 16 / ES, KSTEP = 64 / ES;
+  constexpr int UNROLL = MT == 1 ? 4 : 2;
+  __shared__ f4 part[NW][MT][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int r15 = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const bool n_in = n0 + r15 < p.n;
+  const T* __restrict__ a = static_cast<const T*>(p.a) + (long long)(n_in ? n0 + r15 : 0) * p.lda;
+  const T* __restrict__ b[MT];
+  bool m_in[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    m_in[j] = 16 * j + r15 < p.m;
+    b[j] = static_cast<const T*>(p.b) + (long long)(m_in[j] ? 16 * j + r15 : 0) * p.ldb;
+  }
+  f4 acc[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = wv * KSTEP; k0 < p.k; k0 += UNROLL * NW * KSTEP) {
+    u4 fa[UNROLL], fb[UNROLL][MT];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = k0 + u * NW * KSTEP + g * V;
+      fa[u] = load_piece(a + k, n_in ? p.k - k : 0);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) fb[u][j] = load_piece(b[j] + k, m_in[j] ? p.k - k : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[j] = Mma<T>::step(fa[u], fb[u][j], acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < MT; ++j) part[wv][j][lane] = acc[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * 64; i += 64 * NW) {
+    const int j = i / 64, l = i % 64;
+    f4 s = part[0][j][l];
+    for (int w = 1; w < NW; ++w) s += part[w][j][l];
+    const long long m = 16 * j + (l & 15);
+    const int n = n0 + 4 * (l >> 4);
+    const int left = p.n - n;
+    if (m >= p.m || left <= 0) continue;
+    // four results: half a piece of a two-byte type, so element by element
+    for (int t = 0; t < 4 && t < left; ++t) {
+      float v = s[t];
+      if (p.e.bias) v += bias_at<T>(p.e, n + t);
+      const long long at = m * p.n + n + t;
+      if (p.e.z) static_cast<T*>(p.e.z)[at] = (T)v;
+      v = activate<sizeof(T) == 4>(v, p.e.act);
+      if (p.e.residual) v += (float)static_cast<const T*>(p.e.residual)[m * p.e.residual_stride + n + t];
+      static_cast<T*>(p.e.out)[at] = (T)v;
+    }
+  }
+}
+
+// dz = dy act'(z), rounded to the operands' type for the two products that read it, and the column
+// sums of the unrounded values: workgroup (x, y) takes rows y, y + gridDim.y ... of 64 pieces of 16
+// bytes, four rows at a time (one per wave).  z null: no activation, sums only (dz null too).
+template <class T>
+__global__ __launch_bounds__(256) void lin_dz_kernel(const T* __restrict__ dy, long long dy_stride,
+                                                     const T* __restrict__ z, long long z_stride, int act, int m,
+                                                     int n, T* __restrict__ dz, float* __restrict__ partial) {
+  using namespace lin;
+  constexpr int V = kPer16<T>;
+  __shared__ float cols[4][64 * V];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int c0 = (blockIdx.x * 64 + lane) * V;
+  const int left = n - c0;
+  float sum[V] = {};
+  if (left > 0) {
+    for (long long row = (long long)blockIdx.y * 4 + wv; row < m; row += (long long)gridDim.y * 4) {
+      float g[V];
+      unpack<T>(load_piece(dy + row * dy_stride + c0, left), g);
+      if (z) {
+        float zz[V];
+        unpack<T>(load_piece(z + row * z_stride + c0, left), zz);
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] *= derivative<sizeof(T) == 4>(zz[j], act);
+        store_piece(dz + row * n + c0, pack<T>(g), left);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += g[j];
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) cols[wv][lane * V + j] = sum[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * V; i += 256) {
+    const int c = blockIdx.x * 64 * V + i;
+    if (c < n) partial[(long long)blockIdx.y * n + c] = (cols[0][i] + cols[1][i]) + (cols[2][i] + cols[3][i]);
+  }
+}
+namespace lin {
+constexpr int kCus = 256;  // compute units of an MI355X
+constexpr int kFewRows = 64;
+
+struct Operands {
+  const void* a;
+  long long lda;
+  const void* b;
+  long long ldb;
+  long long n, m, k;
+};
+
+struct Choice {
+  int tile;    // 256, 128, 64
+  int splits;
+  int k_per_split;
+};
+
+static long long tiles_of(long long n, long long m, int tile) {
+  return ((n + tile - 1) / tile) * ((m + tile - 1) / tile);
+}
+
+// The tile and the number of parts of k, from the sizes alone (the workspace size follows from it).
+static Choice choose(long long n, long long m, long long k, size_t es, bool dma) {
+  const int kstep = (int)(64 / es);
+  const long long steps = (k + kstep - 1) / kstep;
+  Choice c{64, 1, 0};
+  if (dma && tiles_of(n, m, 256) >= kCus) c.tile = 256;
+  else if (tiles_of(n, m, 128) >= kCus / 2) c.tile = 128;
+  const long long tiles = tiles_of(n, m, c.tile);
+  const long long fill = c.tile == 256 ? kCus : c.tile == 128 ? 2 * kCus : 4 * kCus;
+  long long splits = 1;
+  if (tiles < fill) splits = fill / tiles;
+  if (splits > steps / 16) splits = steps / 16;
+  if (splits > 32) splits = 32;
+  if (splits < 1) splits = 1;
+  const long long per = steps ? (steps + splits - 1) / splits : 1;
+  c.splits = steps ? (int)((steps + per - 1) / per) : 1;
+  c.k_per_split = (int)(per * kstep);
+  return c;
+}
+
+template <class TL, class T, bool AKC, bool BKC, bool DMA>
+static int launch(Gemm g, hipStream_t s) {
+  g.n_tiles = (g.n + TL::BN - 1) / TL::BN;
+  g.m_tiles = (g.m + TL::BM - 1) / TL::BM;
+  const long long blocks = (long long)g.n_tiles * g.m_tiles * g.splits;
+  if (blocks >= (1LL << 31)) {
+    set_error("product too large for one launch");
+    return MIA_ERR_UNSUPPORTED;
+  }
+  constexpr int lds = DMA ? TL::LDS : 2 * TL::STAGE;
+  auto kern = lin_gemm_kernel<TL, T, AKC, BKC, DMA>;
+  if constexpr (lds > 64 * 1024) {
+    MIA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(TL::WG), lds, s, g);
+  return MIA_OK;
+}
+
+template <class T, bool AKC, bool BKC>
+static int gemm(const Operands& o, const Epilogue& e, void* workspace, bool dma, hipStream_t s) {
+  const Choice c = choose(o.n, o.m, o.k, sizeof(T), dma);
+  Gemm g{o.a, o.b, o.lda, o.ldb, (int)o.n, (int)o.m, (int)o.k, 0, 0, c.splits, c.k_per_split,
+         static_cast<float*>(workspace), e};
+  int rc;
+  if (dma) {
+    rc = c.tile == 256   ? launch<LinTile256, T, AKC, BKC, true>(g, s)
+         : c.tile == 128 ? launch<LinTile128, T, AKC, BKC, true>(g, s)
+                         : launch<LinTile64, T, AKC, BKC, true>(g, s);
+  } else {
+    rc = c.tile == 128 ? launch<LinTile128, T, AKC, BKC, false>(g, s) : launch<LinTile64, T, AKC, BKC, false>(g, s);
+  }
+  if (rc != MIA_OK) return rc;
+  if (c.splits > 1) {
+    const long long work = o.m * ((o.n + 7) / 8);
+    const long long blocks = (work + 255) / 256;
+    hipLaunchKernelGGL(lin_join_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, g);
+  }
+  return MIA_OK;
+}
+
+// 16-byte pieces that are aligned and never cross the operand's edge
+static bool pieces_ok(const void* p, long long ld, long long contiguous, size_t es) {
+  const long long v = (long long)(16 / es);
+  return aligned16(p) && ld % v == 0 && contiguous % v == 0;
+}
+
+static size_t split_bytes(long long n, long long m, long long k, size_t es) {
+  // both ways of loading may be taken (alignment is not known here): the larger of the two
+  size_t most = 0;
+  for (int dma = 0; dma < 2; ++dma) {
+    const Choice c = choose(n, m, k, es, dma != 0);
+    const size_t need = c.splits > 1 ? (size_t)c.splits * m * n * sizeof(float) : 0;
+    most = need > most ? need : most;
+  }
+  return most;
+}
+
+template <class T, int MT>
+static void launch_few(const Gemm& g, hipStream_t s) {
+  const unsigned blocks = (unsigned)((g.n + 15) / 16);
+  hipLaunchKernelGGL((lin_few_kernel<T, MT, 8>), dim3(blocks), dim3(512), 0, s, g);
+}
+template <class T>
+struct Ops {
+  static int forward(const Operands& o, const Epilogue& e, void* workspace, hipStream_t s);
+  static int input_gradient(const Operands& o, const Epilogue& e, void* workspace, hipStream_t s);
+  static int weight_gradient(const Operands& o, const Epilogue& e, void* workspace, hipStream_t s);
+  static void dz(const void* dy, long long dy_stride, const void* z, long long z_stride, int act, long long m,
+                 long long n, void* dz, float* partial, int groups, hipStream_t s);
+};
+#ifdef MIA_LINEAR_TYPE
+template <class T>
+int Ops<T>::forward(const Operands& o, const Epilogue& e, void* workspace, hipStream_t s) {
+  if (o.m <= kFewRows) {
+    const Gemm g{o.a, o.b, o.lda, o.ldb, (int)o.n, (int)o.m, (int)o.k, 0, 0, 1, 0, nullptr, e};
+    if (o.m <= 16) launch_few<T, 1>(g, s);
+    else if (o.m <= 32) launch_few<T, 2>(g, s);
+    else launch_few<T, 4>(g, s);
+    return MIA_OK;
+  }
+  const bool dma = pieces_ok(o.a, o.lda, o.k, sizeof(T)) && pieces_ok(o.b, o.ldb, o.k, sizeof(T));
+  return gemm<T, true, true>(o, e, workspace, dma, s);
+}
+template <class T>
+int Ops<T>::input_gradient(const Operands& o, const Epilogue& e, void* workspace, hipStream_t s) {
+  const bool dma = pieces_ok(o.a, o.lda, o.n, sizeof(T)) && pieces_ok(o.b, o.ldb, o.k, sizeof(T));
+  return gemm<T, false, true>(o, e, workspace, dma, s);
+}
+template <class T>
+int Ops<T>::weight_gradient(const Operands& o, const Epilogue& e, void* workspace, hipStream_t s) {
+  const bool dma = pieces_ok(o.a, o.lda, o.n, sizeof(T)) && pieces_ok(o.b, o.ldb, o.m, sizeof(T));
+  return gemm<T, false, false>(o, e, workspace, dma, s);
+}
+template <class T>
+void Ops<T>::dz(const void* dy, long long dy_stride, const void* z, long long z_stride, int act, long long m,
+                long long n, void* dz, float* partial, int groups, hipStream_t s) {
+  constexpr long long cols = 64 * kPer16<T>;
+  hipLaunchKernelGGL(lin_dz_kernel<T>, dim3((unsigned)((n + cols - 1) / cols), (unsigned)groups), dim3(256), 0, s,
+                     static_cast<const T*>(dy), dy_stride, static_cast<const T*>(z), z_stride, act, (int)m, (int)n,
+                     static_cast<T*>(dz), partial);
+}
+template struct Ops<MIA_LINEAR_TYPE>;
+#endif
+}  // namespace lin
+}  // namespace mia

@@ -1,0 +1,254 @@
+"""The operators of the transformer blocks behind the encoder stem: layer normalisation, the linear
+layer with bias, activation and residual in its epilogue, and attention, each with its backward
+pass (the blocks `AudioEncoder.__call__` runs after the stem, models/whisper/layers/).
+
+Element types are float32, float16 and bfloat16; every sum, statistic and intermediate value is
+float32, and results are rounded once.  Tensors may be views: rows (the last axis) must be
+contiguous and the leading axes of `layer_norm` / `linear` inputs collapse to rows of one stride,
+anything else is copied first.  Host arrays are moved to the GPU.  Work is enqueued on the current
+stream; nothing synchronises, so all functions can be captured into a graph.
+
+These functions record no autograd graph: the gradients come from the `*_backward` functions.
+Inputs that require a gradient are refused while gradients are enabled, so that none is lost
+silently (wrap the calls in `torch.no_grad()`).
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+from .. import _lib
+from .._runtime import require_gpu, stream_ptr
+
+_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_ACTIVATIONS = {None: _lib.ACT_NONE, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH, "relu": _lib.ACT_RELU}
+
+
+def _operands(**given) -> dict:
+    """The given arrays as tensors of a supported type that need no gradient (None stays None)."""
+    out = {}
+    for name, x in given.items():
+        if x is not None and not isinstance(x, torch.Tensor):
+            x = torch.as_tensor(np.asarray(x))
+        if x is not None:
+            if x.dtype not in _DTYPES:
+                raise ValueError(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
+            if x.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError(f"{name} requires a gradient, which this function does not record: call the "
+                                   "*_backward function for it, under torch.no_grad()")
+        out[name] = x
+    return out
+
+
+def _same_type(ops: dict, names) -> torch.dtype:
+    kinds = {n: ops[n].dtype for n in names if ops[n] is not None}
+    if len(set(kinds.values())) != 1:
+        raise ValueError("expected one type, got " + ", ".join(f"{n} {t}" for n, t in kinds.items()))
+    return next(iter(kinds.values()))
+
+
+def _to_device(ops: dict) -> torch.device:
+    """Moves host tensors to the device of the others (the current one if all are host tensors)."""
+    require_gpu()
+    devices = {x.device for x in ops.values() if x is not None and x.is_cuda}
+    if len(devices) > 1:
+        raise ValueError(f"tensors on different devices: {sorted(str(d) for d in devices)}")
+    device = devices.pop() if devices else torch.device("cuda", torch.cuda.current_device())
+    for name, x in ops.items():
+        if x is not None and x.device != device:
+            ops[name] = x.to(device)
+    return device
+
+
+def _rows(x: torch.Tensor):
+    """x as (tensor, rows, row stride): last axis contiguous, leading axes collapsed."""
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty((math.prod(x.shape[:-1]), x.shape[-1]))
+    return x, x.shape[0], (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+
+
+def _ptr(x):
+    return None if x is None else x.data_ptr()
+
+
+def _check_vector(x, name: str, n: int, dtype: torch.dtype) -> None:
+    if x is None:
+        return
+    if tuple(x.shape) != (n,):
+        raise ValueError(f"{name} must have shape ({n},), got {tuple(x.shape)}")
+    if x.dtype not in (dtype, torch.float32):
+        raise ValueError(f"{name} must be float32 or {dtype}, got {x.dtype}")
+
+
+def _check_norm(x, weight, bias) -> None:
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must have a last axis of at least one element, got shape {tuple(x.shape)}")
+    _check_vector(weight, "weight", x.shape[-1], x.dtype)
+    _check_vector(bias, "bias", x.shape[-1], x.dtype)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"expected one type, got weight {weight.dtype}, bias {bias.dtype}")
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool = False):
+    """Layer normalisation over the last axis: (x - mean) / sqrt(variance + eps) * weight + bias.
+
+    x [..., D] -> y [..., D] of x's type; weight and bias [D], float32 or x's type, either may be
+    None.  With return_stats also the rows' mean and 1 / sqrt(variance + eps), float32 [...], which
+    `layer_norm_backward` takes.  One launch that reads x once.
+    """
+    ops = _operands(x=x, weight=weight, bias=bias)
+    _check_norm(ops["x"], ops["weight"], ops["bias"])
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative (got {eps})")
+    device = _to_device(ops)
+    x, w, b = ops["x"], ops["weight"], ops["bias"]
+    w, b = (None if v is None else v.contiguous() for v in (w, b))
+    flat, rows, stride = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    mean = rstd = None
+    if return_stats:
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+        rstd = torch.empty_like(mean)
+    params = next((v for v in (w, b) if v is not None), flat)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().mia_layer_norm(flat.data_ptr(), rows, x.shape[-1], stride, _DTYPES[x.dtype], _ptr(w),
+                                             _ptr(b), _DTYPES[params.dtype], float(eps), y.data_ptr(),
+                                             _ptr(mean) if rows else None, _ptr(rstd) if rows else None,
+                                             stream_ptr(device)))
+    return (y, mean, rstd) if return_stats else y
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None):
+    """Gradients of `layer_norm` from the statistics its forward call returned.
+
+    dy and x [..., D] of one type -> (dx of that type, dweight, dbias): the vectors are sums over
+    all rows and stay in float32; without a weight they are None (a bias alone has the gradient
+    dy summed over its rows).  The sums have a fixed order: two calls give the same bits.
+    """
+    ops = _operands(dy=dy, x=x, mean=mean, rstd=rstd, weight=weight)
+    dy, x, mean, rstd, weight = (ops[n] for n in ("dy", "x", "mean", "rstd", "weight"))
+    _check_norm(x, weight, None)
+    _same_type(ops, ("dy", "x"))
+    if dy.shape != x.shape:
+        raise ValueError(f"dy must have x's shape {tuple(x.shape)}, got {tuple(dy.shape)}")
+    for name in ("mean", "rstd"):
+        if ops[name].dtype != torch.float32 or ops[name].shape != x.shape[:-1]:
+            raise ValueError(f"{name} must be float32 of shape {tuple(x.shape[:-1])}, "
+                             f"got {ops[name].dtype} {tuple(ops[name].shape)}")
+    device = _to_device(ops)
+    flat, rows, stride = _rows(ops["x"])
+    gflat, _, gstride = _rows(ops["dy"])
+    mean, rstd = ops["mean"].contiguous(), ops["rstd"].contiguous()
+    w = None if weight is None else ops["weight"].contiguous()
+    dim = x.shape[-1]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    dw = db = ws = None
+    lib = _lib.lib()
+    need = 0
+    if w is not None:
+        dw = torch.empty((dim,), dtype=torch.float32, device=device)
+        db = torch.empty_like(dw)
+        need = lib.mia_layer_norm_backward_workspace_bytes(rows, dim)
+        ws = torch.empty((need,), dtype=torch.uint8, device=device)
+    with torch.cuda.device(device):
+        _lib.check(lib.mia_layer_norm_backward(gflat.data_ptr(), gstride, flat.data_ptr(), stride, mean.data_ptr(),
+                                               rstd.data_ptr(), rows, dim, _DTYPES[x.dtype], _ptr(w),
+                                               _DTYPES[(flat if w is None else w).dtype], dx.data_ptr(), _ptr(dw),
+                                               _ptr(db), _ptr(ws), need, stream_ptr(device)))
+    return dx, dw, db
+
+
+def _check_linear(x, weight, activation) -> None:
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"Unknown activation: {activation!r}. Supported: None, 'gelu', 'gelu_tanh', 'relu'")
+    if weight.dim() != 2 or min(weight.shape) < 1:
+        raise ValueError(f"weight must be (out, in) with at least one element each, got {tuple(weight.shape)}")
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x must have a last axis of {weight.shape[1]} elements, got shape {tuple(x.shape)}")
+
+
+def linear(x, weight, bias=None, activation=None, residual=None, return_preactivation: bool = False):
+    """The linear layer with its epilogue: activation(x @ weight.T + bias) + residual.
+
+    x [..., in], weight [out, in], residual [..., out] of one type; bias [out] of that type or
+    float32.  activation: None, "gelu" (erf), "gelu_tanh" or "relu".  Returns y [..., out] of x's
+    type; with return_preactivation also x @ weight.T + bias, which `linear_backward` takes.
+    Products of two-byte types accumulate in float32 on the matrix cores; float32 runs on the
+    float32 matrix instruction.
+    """
+    ops = _operands(x=x, weight=weight, bias=bias, residual=residual)
+    x, weight, bias, residual = (ops[n] for n in ("x", "weight", "bias", "residual"))
+    _check_linear(x, weight, activation)
+    dtype = _same_type(ops, ("x", "weight", "residual"))
+    n, k = weight.shape
+    _check_vector(bias, "bias", n, dtype)
+    shape = x.shape[:-1] + (n,)
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must have shape {tuple(shape)}, got {tuple(residual.shape)}")
+    device = _to_device(ops)
+    flat, rows, stride = _rows(ops["x"])
+    w, _, wstride = _rows(ops["weight"])
+    b = None if bias is None else ops["bias"].contiguous()
+    r, rstride = None, 0
+    if residual is not None:
+        r, _, rstride = _rows(ops["residual"])
+    y = torch.empty(shape, dtype=dtype, device=device)
+    z = torch.empty_like(y) if return_preactivation else None
+    lib = _lib.lib()
+    need = lib.mia_linear_workspace_bytes(rows, k, n, _DTYPES[dtype])
+    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    with torch.cuda.device(device):
+        _lib.check(lib.mia_linear(flat.data_ptr(), stride, w.data_ptr(), wstride, _ptr(b),
+                                  _DTYPES[(flat if b is None else b).dtype], _ptr(r), rstride,
+                                  _ACTIVATIONS[activation], rows, k, n, _DTYPES[dtype], y.data_ptr(), _ptr(z),
+                                  _ptr(ws), need, stream_ptr(device)))
+    return (y, z) if return_preactivation else y
+
+
+def linear_backward(dy, x, weight, activation=None, preactivation=None, input_grad: bool = True,
+                    weight_grad: bool = True, bias_grad: bool = True):
+    """Gradients of `linear`: with dz = dy * activation'(preactivation),
+    (dx = dz @ weight, dweight = dz.T @ x, dbias = dz summed over its rows).
+
+    dy [..., out], x [..., in], weight [out, in] and preactivation [..., out] (what the forward call
+    returned; needed for an activation) of one type.  dx and dweight have that type, dbias is
+    float32; a gradient not asked for is None.  The residual's gradient is dy itself.  For the two
+    products dz is rounded to the operands' type.
+    """
+    ops = _operands(dy=dy, x=x, weight=weight, preactivation=preactivation)
+    dy, x, weight, z = (ops[n] for n in ("dy", "x", "weight", "preactivation"))
+    _check_linear(x, weight, activation)
+    dtype = _same_type(ops, ("dy", "x", "weight", "preactivation"))
+    n, k = weight.shape
+    shape = x.shape[:-1] + (n,)
+    if dy.shape != shape:
+        raise ValueError(f"dy must have shape {tuple(shape)}, got {tuple(dy.shape)}")
+    if activation is not None:
+        if z is None:
+            raise ValueError("the backward pass of an activation needs the preactivation")
+        if z.shape != shape:
+            raise ValueError(f"preactivation must have shape {tuple(shape)}, got {tuple(z.shape)}")
+    device = _to_device(ops)
+    flat, rows, stride = _rows(ops["x"])
+    w, _, wstride = _rows(ops["weight"])
+    g, _, gstride = _rows(ops["dy"])
+    zf, zstride = None, 0
+    if activation is not None:
+        zf, _, zstride = _rows(ops["preactivation"])
+    dx = torch.empty(x.shape, dtype=dtype, device=device) if input_grad else None
+    dw = torch.empty((n, k), dtype=dtype, device=device) if weight_grad else None
+    db = torch.empty((n,), dtype=torch.float32, device=device) if bias_grad else None
+    lib = _lib.lib()
+    act = _ACTIVATIONS[activation]
+    need = lib.mia_linear_backward_workspace_bytes(rows, k, n, _DTYPES[dtype], act)
+    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    with torch.cuda.device(device):
+        _lib.check(lib.mia_linear_backward(g.data_ptr(), gstride, flat.data_ptr(), stride, w.data_ptr(), wstride,
+                                           _ptr(zf), zstride, act, rows, k, n, _DTYPES[dtype],
+                                           _ptr(dx) if rows else None, _ptr(dw), _ptr(db), _ptr(ws), need,
+                                           stream_ptr(device)))
+    return dx, dw, db
