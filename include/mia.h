@@ -616,6 +616,36 @@ int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_
                         int64_t rows, int64_t in, int64_t out, int dtype, void* dx, void* dweight, float* dbias,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* out = softmax(scale q k^T) v for every batch item and head; query head h uses key head
+ * h / (heads / kv_heads).  q: [batch, queries, heads, dim], k and v: [batch, keys, kv_heads, dim] by
+ * strides (batch, row, head), dim contiguous, dim <= 128.  key_lengths: device int32 (batch) or NULL:
+ * keys at and behind it are not seen and not read (values are brought into 0 .. keys); causal: query
+ * i sees keys j <= i + keys - queries.  A query that sees no key has out 0 and lse -inf.  out:
+ * contiguous [batch, queries, heads, dim] of q's type; lse: float32 (batch, heads, queries), the
+ * logarithm of the sum of exponentials, or NULL (the backward pass needs it).  A value that is not
+ * finite in a key or value row that SOME query of a causal call sees may reach other queries.
+ * workspace: mia_attention_workspace_bytes bytes, 16-byte aligned (0 unless the keys are split). */
+typedef struct mia_attention_desc {
+  int dtype;
+  int64_t batch, queries, keys;
+  int heads, kv_heads, dim;
+  int causal;
+  float scale;
+  int64_t stride_q[3], stride_k[3], stride_v[3]; /* batch, row, head; in elements */
+} mia_attention_desc;
+size_t mia_attention_workspace_bytes(const mia_attention_desc* desc);
+int mia_attention(const mia_attention_desc* desc, const void* q, const void* k, const void* v,
+                  const int32_t* key_lengths, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                  void* stream);
+/* The gradients, with the probabilities recomputed from lse: dq [batch, queries, heads, dim], dk and
+ * dv [batch, keys, kv_heads, dim] (summed over the query heads that share a key head; zero behind a
+ * length), contiguous.  out and lse are what the forward call wrote; dout and out by strides. */
+size_t mia_attention_backward_workspace_bytes(const mia_attention_desc* desc);
+int mia_attention_backward(const mia_attention_desc* desc, const void* dout, const int64_t* stride_dout,
+                           const void* q, const void* k, const void* v, const void* out, const int64_t* stride_out,
+                           const float* lse, const int32_t* key_lengths, void* dq, void* dk, void* dv,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -49,6 +49,17 @@ class PlanDesc(ctypes.Structure):
     ]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int),
+        ("batch", c_int64), ("queries", c_int64), ("keys", c_int64),
+        ("heads", c_int), ("kv_heads", c_int), ("dim", c_int),
+        ("causal", c_int),
+        ("scale", c_float),
+        ("stride_q", c_int64 * 3), ("stride_k", c_int64 * 3), ("stride_v", c_int64 * 3),
+    ]
+
+
 # name -> (restype, argtypes); must list every symbol include/mia.h declares.
 SIGNATURES = {
     "mia_last_error": (c_char_p, []),
@@ -187,6 +198,13 @@ SIGNATURES = {
     "mia_linear_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int,
                                     c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_size_t, c_void_p]),
+    "mia_attention_workspace_bytes": (c_size_t, [POINTER(AttentionDesc)]),
+    "mia_attention": (c_int, [POINTER(AttentionDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_size_t, c_void_p]),
+    "mia_attention_backward_workspace_bytes": (c_size_t, [POINTER(AttentionDesc)]),
+    "mia_attention_backward": (c_int, [POINTER(AttentionDesc), c_void_p, POINTER(c_int64), c_void_p, c_void_p,
+                                       c_void_p, c_void_p, POINTER(c_int64), c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 HAS_HIP_EXT: bool = False

@@ -1,0 +1,794 @@
+// Attention for the transformer blocks behind the encoder stem, forward and backward.
+//
+//   s = scale q k^T (masked), lse = log sum exp s, out = exp(s - lse) v
+//   p = exp(s - lse), dp = dout v^T, delta = sum_d dout out, ds = p (dp - delta)
+//   dv = p^T dout, dk = scale ds^T q, dq = scale ds k
+//
+// No kernel keeps s or p in memory: the forward runs over the keys once with a running maximum and
+// sum, the backward recomputes p from lse.  Every kernel has the same shape.  A wave OWNS 16 or 32
+// rows (queries in the forward and in dq, keys in dk / dv) whose vectors stay in registers as the
+// second operand of the matrix instruction; the other side's rows STREAM through LDS in tiles that
+// all four waves of the workgroup share.  A product tile then has the own rows as its columns:
+// lane l holds column l & 15 and the stream rows 4 (l >> 4) + i of each 16 - which is, for two such
+// blocks (one for float), exactly the operand layout of the next product's second operand if the
+// sum over stream rows is taken in that order.  So p and ds go from one product into the next
+// without leaving their registers; only the first operand (v, k, dout, q by columns) is read from
+// LDS down the columns (ds_read_b64_tr_b16; float: ds_read_b32).  Row maxima and sums need two lane
+// exchanges.  dk / dv and dq are two launches: one launch would need atomics for dq, whose order
+// changes its bits.
+#pragma once
+#include "nn_common.h"
+
+namespace mia {
+namespace att {
+using namespace nn;
+
+struct View {  // [batch, row, head, dim], dim contiguous, strides in elements
+  const void* p;
+  long long b, s, h;
+};
+struct Args {
+  View q, k, v, out, dout;
+  void* o0;           // forward: out; dq; dk          (contiguous [batch, row, head, dim])
+  void* o1;           // dv
+  float* lse;         // (batch, heads, sq): written by the forward
+  const float* stats; // backward: lse / ln 2 (+inf for an empty row), then delta, (batch, heads, sq) each
+  const int* lengths; // (batch) keys of each batch item, or null
+  int batch, sq, sk, heads, kv_heads, dim;
+  int pack;           // heads that share a workgroup's rows: 1, or heads / kv_heads (few queries)
+  int causal;         // query i sees keys <= i + sk - sq
+  float scale;
+  int own_tiles;      // workgroups along the own rows
+  int splits;         // forward: parts of the keys
+  int keys_per_split;
+  float* partial;     // forward, splits > 1: (splits, rows, dim) sums, then (splits, rows, 2) max and sum
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kInf = __builtin_huge_valf();
+__device__ const u4 kZeros[1] = {};
+__device__ const float kInfinity[1] = {kInf};
+
+template <class T, int DP>
+struct Shape {
+  static constexpr int ES = (int)sizeof(T), V = 16 / ES;
+  static constexpr int TILE = ES == 2 ? 64 : 32;   // stream rows of a tile
+  static constexpr int PITCH = DP * ES;            // bytes of an LDS row
+  static constexpr int PIECES = PITCH / 16;
+  static constexpr int CC = PITCH / 64;            // matrix steps along dim
+  static constexpr int DT = DP / 16;               // accumulators along dim
+  static constexpr int RB = ES == 2 ? 2 : 1;       // 16-row blocks of one matrix step along stream rows
+  static constexpr int BYTES = TILE * PITCH;
+  static constexpr int PW = BYTES / 4096;          // 1 KiB pieces per wave and tile
+};
+
+// Piece c of row r lies at position c ^ (r & 7): rows read side by side fall on different banks.
+// 16 bytes of 16 rows: row block `rb`, piece 4 cc + (lane >> 4)
+template <class T, int DP>
+__device__ __forceinline__ u4 rows_fragment(const unsigned char* tile, int rb, int cc, int lane) {
+  using S = Shape<T, DP>;
+  const int row = 16 * rb + (lane & 15), c = 4 * cc + (lane >> 4);
+  return *reinterpret_cast<const u4*>(tile + row * S::PITCH + ((c ^ (row & 7)) << 4));
+}
+// Columns: lane's column is d = 64 (dt / 4) + 16 (r >> 2) + 4 (dt % 4) + (r & 3), r = lane & 15 (so that
+// four accumulators of a lane group hold 16 consecutive d), its elements are the stream rows of step
+// `st` in the order of the product tiles: rows 4 (lane >> 4) + i of each 16-row block.
+template <class T, int DP>
+__device__ __forceinline__ u4 columns_fragment(const unsigned char* tile, int st, int dt, int lane) {
+  using S = Shape<T, DP>;
+  const int r = lane & 15, g = lane >> 4;
+  if constexpr (S::ES == 2) {
+    const int row = 32 * st + 4 * g + (r >> 2);
+    const int d = 64 * (dt >> 2) + 16 * (r & 3) + 4 * (dt & 3);
+    const unsigned at = (unsigned)(unsigned long long)tile + row * S::PITCH + (((d >> 3) ^ (row & 7)) << 4) + (d & 7) * 2;
+    union {
+      s4 h[2];
+      u4 u;
+    } x;
+    x.h[0] = lds_read_column4(at);
+    x.h[1] = lds_read_column4(at + 16 * S::PITCH);
+    return x.u;
+  } else {
+    const int d = 64 * (dt >> 2) + 16 * (r >> 2) + 4 * (dt & 3) + (r & 3);
+    u4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * st + 4 * g + i;
+      x[i] = *reinterpret_cast<const unsigned*>(tile + row * S::PITCH + (((d >> 2) ^ (row & 7)) << 4) + (d & 3) * 4);
+    }
+    return x;
+  }
+}
+// the product tiles of one step as the next product's second operand
+template <class T>
+__device__ __forceinline__ u4 to_operand(const f4* blocks) {
+  if constexpr (sizeof(T) == 2) {
+    const float v[8] = {blocks[0][0], blocks[0][1], blocks[0][2], blocks[0][3],
+                        blocks[1][0], blocks[1][1], blocks[1][2], blocks[1][3]};
+    return pack<T>(v);
+  } else {
+    return __builtin_bit_cast(u4, blocks[0]);
+  }
+}
+
+// Loads tiles of stream rows; rows at or past `end` and elements past dim read as zero whatever
+// memory holds there.  DMA: straight into LDS (pieces aligned, dim a whole number of them); else
+// through registers.
+template <class T, int DP, bool DMA>
+struct Loader {
+  using S = Shape<T, DP>;
+  u4 held[DMA ? 1 : S::PW];
+  __device__ __forceinline__ void issue(const void* base, long long stride, int row0, int end, int dim, unsigned lds,
+                                        int wv, int lane) {
+#pragma unroll
+    for (int i = 0; i < S::PW; ++i) {
+      const int s = (S::PW * wv + i) * 64 + lane;
+      const int r = s / S::PIECES, c = (s % S::PIECES) ^ (r & 7);
+      const int row = row0 + r;
+      const T* from = static_cast<const T*>(base) + (long long)row * stride + c * S::V;
+      if constexpr (DMA) {
+        const void* src = row < end && c * S::V < dim ? static_cast<const void*>(from) : static_cast<const void*>(kZeros);
+        dma16(src, (unsigned)__builtin_amdgcn_readfirstlane((int)(lds + (unsigned)(S::PW * wv + i) * 1024u)));
+      } else {
+        held[i] = u4{0, 0, 0, 0};
+        if (row < end && c * S::V < dim) held[i] = load_piece(from, dim - c * S::V);
+      }
+    }
+  }
+  __device__ __forceinline__ void commit(unsigned char* tile, int wv, int lane) {
+    if constexpr (!DMA) {
+#pragma unroll
+      for (int i = 0; i < S::PW; ++i)
+        *reinterpret_cast<u4*>(tile + ((S::PW * wv + i) * 64 + lane) * 16) = held[i];
+    }
+  }
+};
+
+// An own row's vector as the second operand: step cc, elements V (4 cc + (lane >> 4)) ...
+template <class T, int DP>
+__device__ __forceinline__ void load_own(const T* row, bool in, int dim, int lane, u4* out) {
+  using S = Shape<T, DP>;
+#pragma unroll
+  for (int cc = 0; cc < S::CC; ++cc) {
+    const int e = (4 * cc + (lane >> 4)) * S::V;
+    out[cc] = u4{0, 0, 0, 0};
+    if (in && e < dim) out[cc] = load_piece(row + e, dim - e);
+  }
+}
+// 16 consecutive values of a lane: accumulators 4 grp .. 4 grp + 3 of own column `c`
+template <class T, int DT, int N>
+__device__ __forceinline__ void store_own(T* row, int dim, int lane, const f4 (&acc)[DT][N], int c, float factor) {
+  constexpr int V = kPer16<T>;
+#pragma unroll
+  for (int grp = 0; grp < DT / 4; ++grp) {
+    const int d = 64 * grp + 16 * (lane >> 4);
+    float v[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) v[t] = acc[4 * grp + t / 4][c][t % 4] * factor;
+#pragma unroll
+    for (int j = 0; j < 16; j += V) store_piece(row + d + j, pack<T>(v + j), dim - d - j);
+  }
+}
+
+// Workgroups that share a batch item and head follow each other on one XCD.
+__device__ __forceinline__ unsigned xcd_order() {
+  const unsigned nb = gridDim.x, id = blockIdx.x, q8 = nb / 8, r8 = nb % 8, xcd = id % 8;
+  return (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + id / 8;
+}
+__device__ __forceinline__ int keys_of(const Args& p, int b) {
+  return p.lengths ? min(max(p.lengths[b], 0), p.sk) : p.sk;
+}
+// sum / maximum over the four lanes that hold a column
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+}  // namespace att
+
+// Forward.  OT: blocks of 16 queries per wave.
+template <class T, int DP, int OT, bool DMA>
+__global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
+  using namespace att;
+  using S = Shape<T, DP>;
+  constexpr int KB = S::TILE / 16, STEPS = KB / S::RB;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * S::BYTES];  // two buffers of k and v
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4;
+
+  unsigned id = xcd_order();
+  const int split = (int)(id % (unsigned)p.splits);
+  id /= (unsigned)p.splits;
+  const int tile = (int)(id % (unsigned)p.own_tiles);
+  id /= (unsigned)p.own_tiles;
+  const int hgs = p.heads / p.pack;
+  const int hg = (int)(id % (unsigned)hgs), b = (int)(id / (unsigned)hgs);
+  const int kvh = hg * p.pack / (p.heads / p.kv_heads);
+  const int rows = p.sq * p.pack;
+  const int row0 = tile * (64 * OT) + wv * (16 * OT);
+  const int off = p.sk - p.sq;
+  const float c = p.scale * kLog2e;
+
+  int len = keys_of(p, b);
+  int k_begin = split * p.keys_per_split;
+  int k_end = min(len, k_begin + p.keys_per_split);
+  const int first_row = tile * (64 * OT), last_row = min(rows, first_row + 64 * OT) - 1;
+  if (p.causal) {  // the furthest key that a row of this workgroup sees
+    const int far = first_row / p.sq == last_row / p.sq ? last_row % p.sq : p.sq - 1;
+    k_end = min(k_end, far + off + 1);
+  }
+
+  u4 own[OT][S::CC];
+  int limit[OT];  // keys that the lane's query sees
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int r = row0 + 16 * o + (lane & 15);
+    const bool in = r < rows;
+    const int hl = in ? r / p.sq : 0, s = in ? r - hl * p.sq : 0;
+    load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + (hg * p.pack + hl) * p.q.h, in, p.dim, lane,
+                    own[o]);
+    limit[o] = p.causal ? min(len, s + off + 1) : len;
+  }
+  // every key before this one is seen by all of the wave's rows
+  int open = len;
+  if (p.causal) {
+    const int last = min(rows, row0 + 16 * OT) - 1;
+    const int near = row0 < rows && row0 / p.sq == last / p.sq ? row0 % p.sq : 0;
+    open = min(len, near + off + 1);
+  }
+
+  f4 acc[S::DT][OT];
+  float mx[OT], sum[OT];
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    mx[o] = -kInf, sum[o] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) acc[d][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const T* kp = static_cast<const T*>(p.k.p) + b * p.k.b + kvh * p.k.h;
+  const T* vp = static_cast<const T*>(p.v.p) + b * p.v.b + kvh * p.v.h;
+  const unsigned lds0 = (unsigned)(unsigned long long)smem;
+  Loader<T, DP, DMA> lk, lv;
+  const int tiles = k_end > k_begin ? (k_end - k_begin + S::TILE - 1) / S::TILE : 0;
+  if (tiles) {
+    lk.issue(kp, p.k.s, k_begin, k_end, p.dim, lds0, wv, lane);
+    lv.issue(vp, p.v.s, k_begin, k_end, p.dim, lds0 + S::BYTES, wv, lane);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    unsigned char* kt = smem + (t & 1) * 2 * S::BYTES;
+    unsigned char* vt = kt + S::BYTES;
+    lk.commit(kt, wv, lane);
+    lv.commit(vt, wv, lane);
+    wait_loads<0>();
+    barrier_keep_loads();  // tile t is there, and nobody reads the other buffer any more
+    const int k0 = k_begin + t * S::TILE;
+    if (t + 1 < tiles) {
+      const unsigned next = lds0 + ((t + 1) & 1) * 2 * S::BYTES;
+      lk.issue(kp, p.k.s, k0 + S::TILE, k_end, p.dim, next, wv, lane);
+      lv.issue(vp, p.v.s, k0 + S::TILE, k_end, p.dim, next + S::BYTES, wv, lane);
+    }
+    if (row0 >= rows) continue;
+
+    f4 s[KB][OT];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int o = 0; o < OT; ++o) s[kb][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int cc = 0; cc < S::CC; ++cc)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const u4 f = rows_fragment<T, DP>(kt, kb, cc, lane);
+#pragma unroll
+        for (int o = 0; o < OT; ++o) s[kb][o] = Mma<T>::step(f, own[o][cc], s[kb][o]);
+      }
+    if (k0 + S::TILE > min(open, k_end)) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int o = 0; o < OT; ++o)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[kb][o][i] = k0 + 16 * kb + 4 * g + i < min(limit[o], k_end) ? s[kb][o][i] : -kInf;
+    }
+#pragma unroll
+    for (int o = 0; o < OT; ++o) {
+      float m = s[0][o][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, s[kb][o][i]);
+      m = fmaxf(mx[o], column_max(m));
+      const float ms = m == -kInf ? 0.0f : m * c;  // a row that has seen nothing yet: exp2(-inf) = 0
+      if (__any(m > mx[o])) {
+        const float alpha = exp2_fast(fmaf(mx[o], c, -ms));
+        mx[o] = m;
+        sum[o] *= alpha;
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) acc[d][o] *= alpha;
+      }
+      float part = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = exp2_fast(fmaf(s[kb][o][i], c, -ms));
+          s[kb][o][i] = e;
+          part += e;
+        }
+      sum[o] += part;
+    }
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      u4 pf[OT];
+#pragma unroll
+      for (int o = 0; o < OT; ++o) {
+        f4 blocks[S::RB];
+#pragma unroll
+        for (int r = 0; r < S::RB; ++r) blocks[r] = s[st * S::RB + r][o];
+        pf[o] = to_operand<T>(blocks);
+      }
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        const u4 f = columns_fragment<T, DP>(vt, st, d, lane);
+#pragma unroll
+        for (int o = 0; o < OT; ++o) acc[d][o] = Mma<T>::step(f, pf[o], acc[d][o]);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int r = row0 + 16 * o + (lane & 15);
+    if (r >= rows) continue;   // (its other three lanes leave too)
+    const float total = column_sum(sum[o]);
+    const int hl = r / p.sq, s = r - hl * p.sq, h = hg * p.pack + hl;
+    const long long at = ((long long)b * p.heads + h) * p.sq + s;
+    if (p.splits > 1) {
+      const long long n = (long long)p.batch * p.heads * p.sq, row = split * n + at;
+      store_own<float>(p.partial + row * p.dim, p.dim, lane, acc, o, 1.0f);
+      if (g == 0) {
+        float* ml = p.partial + (long long)p.splits * n * p.dim + row * 2;
+        ml[0] = mx[o] * c;
+        ml[1] = total;
+      }
+    } else {
+      // an empty row (sum 0) is zero; a NaN in the sum stays one
+      store_own<T>(static_cast<T*>(p.o0) + (((long long)b * p.sq + s) * p.heads + h) * p.dim, p.dim, lane, acc, o,
+                   total == 0.0f ? 0.0f : 1.0f / total);
+      if (g == 0 && p.lse) p.lse[at] = total == 0.0f ? -kInf : fmaf(mx[o], p.scale, logf(total));
+    }
+  }
+}
+
+// The parts of a row that was split along the keys: one wave per row.
+template <class T>
+__global__ __launch_bounds__(256) void att_join_kernel(att::Args p) {
+  using namespace att;
+  const long long n = (long long)p.batch * p.heads * p.sq;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (at >= n) return;
+  const float* __restrict__ ml = p.partial + (long long)p.splits * n * p.dim;
+  float top = -kInf;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[(s * n + at) * 2]);
+  const float base = top == -kInf ? 0.0f : top;
+  float total = 0.0f, v[2] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const long long row = s * n + at;
+    const float w = exp2_fast(ml[row * 2] - base);
+    total = fmaf(w, ml[row * 2 + 1], total);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (lane + 64 * j < p.dim) v[j] = fmaf(w, p.partial[row * p.dim + lane + 64 * j], v[j]);
+  }
+  const long long bh = at / p.sq;
+  const int s = (int)(at - bh * p.sq), h = (int)(bh % p.heads);
+  const long long b = bh / p.heads;
+  T* out = static_cast<T*>(p.o0) + ((b * p.sq + s) * p.heads + h) * p.dim;
+  const float f = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (lane + 64 * j < p.dim) out[lane + 64 * j] = (T)(v[j] * f);
+  if (lane == 0 && p.lse) p.lse[at] = total == 0.0f ? -kInf : fmaf(top, kLn2, logf(total));
+}
+
+// stats[0] = lse / ln 2 (+inf for an empty row: its p becomes 0), stats[1] = delta = sum_d dout out.
+// 16 lanes per row, rows in memory order.
+template <class T>
+__global__ __launch_bounds__(256) void att_stats_kernel(att::Args p, const float* __restrict__ lse,
+                                                        float* __restrict__ stats) {
+  using namespace att;
+  constexpr int V = kPer16<T>;
+  const long long n = (long long)p.batch * p.heads * p.sq;
+  const long long r = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int l = threadIdx.x & 15;
+  if (r >= n) return;
+  const int h = (int)(r % p.heads);
+  const long long bs = r / p.heads, b = bs / p.sq;
+  const int s = (int)(bs - b * p.sq);
+  const T* o = static_cast<const T*>(p.out.p) + b * p.out.b + s * p.out.s + h * p.out.h;
+  const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.b + s * p.dout.s + h * p.dout.h;
+  float d = 0.0f;
+  for (int e = l * V; e < p.dim; e += 16 * V) {
+    float x[V], y[V];
+    unpack<T>(load_piece(o + e, p.dim - e), x);
+    unpack<T>(load_piece(g + e, p.dim - e), y);
+#pragma unroll
+    for (int j = 0; j < V; ++j) d = fmaf(x[j], y[j], d);
+  }
+#pragma unroll
+  for (int k = 8; k; k >>= 1) d += __shfl_xor(d, k);
+  if (l == 0) {
+    const long long at = (b * p.heads + h) * p.sq + s;
+    const float v = lse[at];
+    stats[at] = v == -kInf ? kInf : v * kLog2e;
+    stats[n + at] = d;
+  }
+}
+
+// dq: own rows are queries, k and v stream.
+template <class T, int DP, int OT, bool DMA>
+__global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
+  using namespace att;
+  using S = Shape<T, DP>;
+  constexpr int STEPS = S::TILE / 16 / S::RB;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * S::BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4;
+  unsigned id = xcd_order();
+  const int tile = (int)(id % (unsigned)p.own_tiles);
+  id /= (unsigned)p.own_tiles;
+  const int h = (int)(id % (unsigned)p.heads), b = (int)(id / (unsigned)p.heads);
+  const int kvh = h / (p.heads / p.kv_heads);
+  const int row0 = tile * (64 * OT) + wv * (16 * OT);
+  const int off = p.sk - p.sq;
+  const float c = p.scale * kLog2e;
+  const int len = keys_of(p, b);
+  int k_end = len;
+  if (p.causal) k_end = min(k_end, min(p.sq, tile * (64 * OT) + 64 * OT) + off);
+  const int open = p.causal ? min(len, row0 + off + 1) : len;
+
+  const long long n = (long long)p.batch * p.heads * p.sq;
+  u4 oq[OT][S::CC], og[OT][S::CC];
+  float lse2[OT], delta[OT];
+  int limit[OT];
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int s = row0 + 16 * o + (lane & 15);
+    const bool in = s < p.sq;
+    load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + h * p.q.h, in, p.dim, lane, oq[o]);
+    load_own<T, DP>(static_cast<const T*>(p.dout.p) + b * p.dout.b + s * p.dout.s + h * p.dout.h, in, p.dim, lane, og[o]);
+    const long long at = ((long long)b * p.heads + h) * p.sq + s;
+    lse2[o] = in ? p.stats[at] : kInf;
+    delta[o] = in ? p.stats[n + at] : 0.0f;
+    limit[o] = p.causal ? min(len, s + off + 1) : len;
+  }
+  f4 acc[S::DT][OT];
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+    for (int o = 0; o < OT; ++o) acc[d][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const T* kp = static_cast<const T*>(p.k.p) + b * p.k.b + kvh * p.k.h;
+  const T* vp = static_cast<const T*>(p.v.p) + b * p.v.b + kvh * p.v.h;
+  const unsigned lds0 = (unsigned)(unsigned long long)smem;
+  Loader<T, DP, DMA> lk, lv;
+  const int tiles = k_end > 0 ? (k_end + S::TILE - 1) / S::TILE : 0;
+  if (tiles) {
+    lk.issue(kp, p.k.s, 0, k_end, p.dim, lds0, wv, lane);
+    lv.issue(vp, p.v.s, 0, k_end, p.dim, lds0 + S::BYTES, wv, lane);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    unsigned char* kt = smem + (t & 1) * 2 * S::BYTES;
+    unsigned char* vt = kt + S::BYTES;
+    lk.commit(kt, wv, lane);
+    lv.commit(vt, wv, lane);
+    wait_loads<0>();
+    barrier_keep_loads();
+    const int k0 = t * S::TILE;
+    if (t + 1 < tiles) {
+      const unsigned next = lds0 + ((t + 1) & 1) * 2 * S::BYTES;
+      lk.issue(kp, p.k.s, k0 + S::TILE, k_end, p.dim, next, wv, lane);
+      lv.issue(vp, p.v.s, k0 + S::TILE, k_end, p.dim, next + S::BYTES, wv, lane);
+    }
+    if (row0 >= p.sq) continue;
+    const bool masked = k0 + S::TILE > min(open, k_end);
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      f4 s[S::RB][OT], dp[S::RB][OT];
+#pragma unroll
+      for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+        for (int o = 0; o < OT; ++o) s[r][o] = dp[r][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int cc = 0; cc < S::CC; ++cc)
+#pragma unroll
+        for (int r = 0; r < S::RB; ++r) {
+          const u4 fk = rows_fragment<T, DP>(kt, st * S::RB + r, cc, lane);
+          const u4 fv = rows_fragment<T, DP>(vt, st * S::RB + r, cc, lane);
+#pragma unroll
+          for (int o = 0; o < OT; ++o) {
+            s[r][o] = Mma<T>::step(fk, oq[o][cc], s[r][o]);
+            dp[r][o] = Mma<T>::step(fv, og[o][cc], dp[r][o]);
+          }
+        }
+      u4 df[OT];
+#pragma unroll
+      for (int o = 0; o < OT; ++o) {
+        f4 blocks[S::RB];
+#pragma unroll
+        for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float e = exp2_fast(fmaf(s[r][o][i], c, -lse2[o]));
+            if (masked) e = k0 + 16 * (st * S::RB + r) + 4 * g + i < limit[o] ? e : 0.0f;
+            blocks[r][i] = e * (dp[r][o][i] - delta[o]);
+          }
+        df[o] = to_operand<T>(blocks);
+      }
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        const u4 f = columns_fragment<T, DP>(kt, st, d, lane);
+#pragma unroll
+        for (int o = 0; o < OT; ++o) acc[d][o] = Mma<T>::step(f, df[o], acc[d][o]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int s = row0 + 16 * o + (lane & 15);
+    if (s >= p.sq) continue;
+    store_own<T>(static_cast<T*>(p.o0) + (((long long)b * p.sq + s) * p.heads + h) * p.dim, p.dim, lane, acc, o, p.scale);
+  }
+}
+
+// dk and dv: own rows are keys, q and dout stream, over all heads that share the key head.
+template <class T, int DP, int OT, bool DMA>
+__global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_kernel(att::Args p) {
+  using namespace att;
+  using S = Shape<T, DP>;
+  constexpr int STEPS = S::TILE / 16 / S::RB;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * S::BYTES];
+  __shared__ float rows_lse[2][64], rows_delta[2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4;
+  unsigned id = xcd_order();
+  const int tile = (int)(id % (unsigned)p.own_tiles);
+  id /= (unsigned)p.own_tiles;
+  const int kvh = (int)(id % (unsigned)p.kv_heads), b = (int)(id / (unsigned)p.kv_heads);
+  const int group = p.heads / p.kv_heads;
+  const int key0 = tile * (64 * OT), row0 = key0 + wv * (16 * OT);
+  const int off = p.sk - p.sq;
+  const float c = p.scale * kLog2e;
+  const int len = keys_of(p, b);
+
+  u4 ok[OT][S::CC], ov[OT][S::CC];
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int s = row0 + 16 * o + (lane & 15);
+    load_own<T, DP>(static_cast<const T*>(p.k.p) + b * p.k.b + (long long)s * p.k.s + kvh * p.k.h, s < len, p.dim, lane, ok[o]);
+    load_own<T, DP>(static_cast<const T*>(p.v.p) + b * p.v.b + (long long)s * p.v.s + kvh * p.v.h, s < len, p.dim, lane, ov[o]);
+  }
+  f4 dk[S::DT][OT], dv[S::DT][OT];
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+    for (int o = 0; o < OT; ++o) dk[d][o] = dv[d][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // the first query that sees any of these keys; a workgroup past the length has nothing to do
+  const int first = p.causal ? max(0, key0 - off) / S::TILE * S::TILE : 0;
+  const int per_head = key0 < len && first < p.sq ? (p.sq - first + S::TILE - 1) / S::TILE : 0;
+  const int tiles = per_head * group;
+  const long long n = (long long)p.batch * p.heads * p.sq;
+  const unsigned lds0 = (unsigned)(unsigned long long)smem;
+  const unsigned lse_at = (unsigned)(unsigned long long)&rows_lse[0][0];
+  const unsigned delta_at = (unsigned)(unsigned long long)&rows_delta[0][0];
+  Loader<T, DP, DMA> lq, lg;
+  auto issue = [&](int t) {
+    const int h = kvh * group + t / per_head, q0 = first + t % per_head * S::TILE;
+    const unsigned at = lds0 + (t & 1) * 2 * S::BYTES;
+    lq.issue(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.s, q0, p.sq, p.dim, at, wv, lane);
+    lg.issue(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.s, q0, p.sq, p.dim, at + S::BYTES, wv, lane);
+    const bool in = lane < S::TILE && q0 + lane < p.sq;
+    const float* from = p.stats + ((long long)b * p.heads + h) * p.sq + q0 + lane;
+    if (wv == 0) dma4(in ? from : kInfinity, (unsigned)__builtin_amdgcn_readfirstlane((int)(lse_at + (t & 1) * 256u)));
+    if (wv == 1)
+      dma4(in ? from + n : reinterpret_cast<const float*>(kZeros),
+           (unsigned)__builtin_amdgcn_readfirstlane((int)(delta_at + (t & 1) * 256u)));
+  };
+  if (tiles) issue(0);
+  for (int t = 0; t < tiles; ++t) {
+    unsigned char* qt = smem + (t & 1) * 2 * S::BYTES;
+    unsigned char* gt = qt + S::BYTES;
+    lq.commit(qt, wv, lane);
+    lg.commit(gt, wv, lane);
+    wait_loads<0>();
+    barrier_keep_loads();
+    const int q0 = first + t % per_head * S::TILE;
+    if (t + 1 < tiles) issue(t + 1);
+    if (row0 >= len) continue;
+    // rows of this tile at or past `open` see all of the wave's keys
+    const bool masked = row0 + 16 * OT > len || (p.causal && row0 + 16 * OT - 1 > q0 + off);
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      f4 s[S::RB][OT], dp[S::RB][OT];
+#pragma unroll
+      for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+        for (int o = 0; o < OT; ++o) s[r][o] = dp[r][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int cc = 0; cc < S::CC; ++cc)
+#pragma unroll
+        for (int r = 0; r < S::RB; ++r) {
+          const u4 fq = rows_fragment<T, DP>(qt, st * S::RB + r, cc, lane);
+          const u4 fg = rows_fragment<T, DP>(gt, st * S::RB + r, cc, lane);
+#pragma unroll
+          for (int o = 0; o < OT; ++o) {
+            s[r][o] = Mma<T>::step(fq, ok[o][cc], s[r][o]);
+            dp[r][o] = Mma<T>::step(fg, ov[o][cc], dp[r][o]);
+          }
+        }
+      f4 lse2[S::RB], delta[S::RB];
+#pragma unroll
+      for (int r = 0; r < S::RB; ++r) {
+        const int at = 16 * (st * S::RB + r) + 4 * g;
+        lse2[r] = *reinterpret_cast<const f4*>(&rows_lse[t & 1][at]);
+        delta[r] = *reinterpret_cast<const f4*>(&rows_delta[t & 1][at]);
+      }
+      u4 pf[OT], df[OT];
+#pragma unroll
+      for (int o = 0; o < OT; ++o) {
+        f4 pb[S::RB], db[S::RB];
+        const int key = row0 + 16 * o + (lane & 15);
+#pragma unroll
+        for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float e = exp2_fast(fmaf(s[r][o][i], c, -lse2[r][i]));
+            if (masked) {
+              const int q = q0 + 16 * (st * S::RB + r) + 4 * g + i;
+              e = key < len && (!p.causal || key <= q + off) ? e : 0.0f;
+            }
+            pb[r][i] = e;
+            db[r][i] = e * (dp[r][o][i] - delta[r][i]);
+          }
+        pf[o] = to_operand<T>(pb);
+        df[o] = to_operand<T>(db);
+      }
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        const u4 fg = columns_fragment<T, DP>(gt, st, d, lane);
+        const u4 fq = columns_fragment<T, DP>(qt, st, d, lane);
+#pragma unroll
+        for (int o = 0; o < OT; ++o) {
+          dv[d][o] = Mma<T>::step(fg, pf[o], dv[d][o]);
+          dk[d][o] = Mma<T>::step(fq, df[o], dk[d][o]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int s = row0 + 16 * o + (lane & 15);
+    if (s >= p.sk) continue;
+    const long long at = (((long long)b * p.sk + s) * p.kv_heads + kvh) * p.dim;
+    store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, dk, o, p.scale);
+    store_own<T>(static_cast<T*>(p.o1) + at, p.dim, lane, dv, o, 1.0f);
+  }
+}
+
+namespace att {
+constexpr int kCus = 256;
+
+struct Plan {
+  int pack, own_tiles, splits, keys_per_split, own_blocks;
+};
+// Queries: 128 per workgroup (32 per wave), or 64 where that leaves compute units without work; then
+// the keys are split until there are two workgroups per unit.
+static Plan plan_forward(long long batch, long long sq, long long sk, int heads, int kv_heads) {
+  Plan p;
+  const int group = heads / kv_heads;
+  p.pack = sq * group <= 64 ? group : 1;
+  const long long rows = sq * p.pack, outer = batch * (heads / p.pack);
+  p.own_blocks = outer * ((rows + 127) / 128) >= 2 * kCus && rows > 64 ? 2 : 1;
+  p.own_tiles = (int)((rows + 64 * p.own_blocks - 1) / (64 * p.own_blocks));
+  const long long groups = outer * p.own_tiles;
+  long long splits = groups ? (4 * kCus) / groups : 1;
+  const long long most = (sk + 255) / 256;  // at least 256 keys each
+  if (splits > most) splits = most;
+  if (splits > 64) splits = 64;
+  if (splits < 1) splits = 1;
+  long long per = (sk + splits - 1) / splits;
+  per = (per + 63) / 64 * 64;
+  if (per < 64) per = 64;
+  p.splits = (int)((sk + per - 1) / per);
+  if (p.splits < 1) p.splits = 1;
+  p.keys_per_split = (int)per;
+  return p;
+}
+static int own_blocks(long long outer, long long rows) { return outer * ((rows + 127) / 128) >= 2 * kCus && rows > 64 ? 2 : 1; }
+
+template <class T>
+struct Ops {
+  static int forward(Args a, hipStream_t s);
+  static int backward(Args a, const float* lse, float* stats, void* dq, void* dk, void* dv, hipStream_t s);
+};
+#ifdef MIA_ATTENTION_TYPE
+static bool pieces_ok(const View& v, size_t es) {
+  const long long n = (long long)(16 / es);
+  return aligned16(v.p) && v.b % n == 0 && v.s % n == 0 && v.h % n == 0;
+}
+#define MIA_ATT_LAUNCH(kernel, ot, grid)                                                                           \
+  do {                                                                                                             \
+    if (a.dim <= 64) {                                                                                             \
+      if (ot == 2) hipLaunchKernelGGL((kernel<T, 64, 2, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);   \
+      else hipLaunchKernelGGL((kernel<T, 64, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);           \
+    } else {                                                                                                       \
+      if (ot == 2) hipLaunchKernelGGL((kernel<T, 128, 2, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);  \
+      else hipLaunchKernelGGL((kernel<T, 128, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);          \
+    }                                                                                                              \
+  } while (0)
+
+template <class F>
+static void with_dma(bool dma, F f) {
+  if (dma) f(std::true_type());
+  else f(std::false_type());
+}
+
+template <class T>
+int Ops<T>::forward(Args a, hipStream_t s) {
+  const Plan pl = plan_forward(a.batch, a.sq, a.sk, a.heads, a.kv_heads);
+  a.pack = pl.pack, a.own_tiles = pl.own_tiles, a.splits = pl.splits, a.keys_per_split = pl.keys_per_split;
+  const long long grid = (long long)a.batch * (a.heads / a.pack) * a.own_tiles * a.splits;
+  if (grid >= (1LL << 31)) {
+    set_error("too many workgroups for one launch");
+    return MIA_ERR_UNSUPPORTED;
+  }
+  const bool dma = a.dim % (16 / (int)sizeof(T)) == 0 && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T));
+  with_dma(dma, [&](auto dma) { MIA_ATT_LAUNCH(att_fwd_kernel, pl.own_blocks, (unsigned)grid); });
+  if (a.splits > 1) {
+    const long long rows = (long long)a.batch * a.heads * a.sq;
+    hipLaunchKernelGGL(att_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  }
+  return MIA_OK;
+}
+template <class T>
+int Ops<T>::backward(Args a, const float* lse, float* stats, void* dq, void* dk, void* dv, hipStream_t s) {
+  const long long rows = (long long)a.batch * a.heads * a.sq;
+  const bool whole = a.dim % (16 / (int)sizeof(T)) == 0;
+  a.stats = stats, a.splits = 1, a.pack = 1;
+  if (rows) hipLaunchKernelGGL(att_stats_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, lse, stats);
+  if (a.sk) {
+    // (two blocks of keys with vectors of 256 bytes and more would not fit the registers)
+    const int ot = a.dim * (int)sizeof(T) <= 128 ? own_blocks((long long)a.batch * a.kv_heads, a.sk) : 1;
+    a.own_tiles = (a.sk + 64 * ot - 1) / (64 * ot);
+    a.o0 = dk, a.o1 = dv;
+    const unsigned grid = (unsigned)a.batch * (unsigned)a.kv_heads * (unsigned)a.own_tiles;
+    with_dma(whole && pieces_ok(a.q, sizeof(T)) && pieces_ok(a.dout, sizeof(T)),
+             [&](auto dma) {
+               if (ot == 2) hipLaunchKernelGGL((att_dkv_kernel<T, 64, 2, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);
+               else if (a.dim <= 64) hipLaunchKernelGGL((att_dkv_kernel<T, 64, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);
+               else hipLaunchKernelGGL((att_dkv_kernel<T, 128, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);
+             });
+  }
+  if (rows) {
+    const int ot = own_blocks((long long)a.batch * a.heads, a.sq);
+    a.own_tiles = (a.sq + 64 * ot - 1) / (64 * ot);
+    a.o0 = dq, a.o1 = nullptr;
+    const unsigned grid = (unsigned)a.batch * (unsigned)a.heads * (unsigned)a.own_tiles;
+    with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)),
+             [&](auto dma) { MIA_ATT_LAUNCH(att_dq_kernel, ot, grid); });
+  }
+  return MIA_OK;
+}
+template struct Ops<MIA_ATTENTION_TYPE>;
+#endif
+}  // namespace att
+}  // namespace mia

@@ -13,7 +13,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
-SOURCES = ["capi.hip", "ops.hip", "spectral_fwd.hip", "spectral_lane.hip", "spectral_wave.hip", "spectral_inv.hip", "logmel400.hip", "resample.hip", "bigfft.hip", "features.hip", "onset.hip", "griffinlim.hip", "gate.hip", "normalize.hip", "stem.hip", "layernorm.hip", "linear.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip"]
+SOURCES = ["capi.hip", "ops.hip", "spectral_fwd.hip", "spectral_lane.hip", "spectral_wave.hip", "spectral_inv.hip", "logmel400.hip", "resample.hip", "bigfft.hip", "features.hip", "onset.hip", "griffinlim.hip", "gate.hip", "normalize.hip", "stem.hip", "layernorm.hip", "linear.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip", "attention.hip", "attention_f32.hip", "attention_f16.hip", "attention_bf16.hip"]
 LIB = os.path.join(HERE, "libmia_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-slp-vectorize", "-Wall", "-Wno-unused-function"]
 # no packed float32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results

@@ -128,6 +128,19 @@ __device__ __forceinline__ void dma16(const void* gptr, unsigned lds_byte_addr) 
       : "v"(gptr), "s"(lds_byte_addr)
       : "memory");
 }
+// the same with 4 bytes a lane, at lds_byte_addr + 4 L
+__device__ __forceinline__ void dma4(const void* gptr, unsigned lds_byte_addr) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(gptr), "s"(lds_byte_addr)
+      : "memory");
+}
 // all but the newest N of this wave's vector loads have arrived, all its LDS operations are done
 template <int N>
 __device__ __forceinline__ void wait_loads() {

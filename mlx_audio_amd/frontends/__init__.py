@@ -4,7 +4,8 @@ behind Whisper's encoder stem."""
 
 from .clap import CLAPFeatureExtractor, clap_log_mel
 from .demucs import htdemucs_ispec, htdemucs_normalize, htdemucs_spec
-from .transformer import layer_norm, layer_norm_backward, linear, linear_backward
+from .transformer import (attention, attention_backward, layer_norm, layer_norm_backward, linear,
+                          linear_backward)
 from .whisper import (WhisperEncoderStem, compute_log_mel_spectrogram, pad_or_trim, sinusoids,
                       whisper_encoder_stem)
 
@@ -12,4 +13,5 @@ __all__ = [
     "compute_log_mel_spectrogram", "pad_or_trim", "htdemucs_spec", "htdemucs_ispec", "htdemucs_normalize",
     "clap_log_mel", "CLAPFeatureExtractor", "WhisperEncoderStem", "whisper_encoder_stem", "sinusoids",
     "layer_norm", "layer_norm_backward", "linear", "linear_backward",
+    "attention", "attention_backward",
 ]

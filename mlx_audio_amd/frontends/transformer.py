@@ -15,6 +15,7 @@ silently (wrap the calls in `torch.no_grad()`).
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -252,3 +253,123 @@ def linear_backward(dy, x, weight, activation=None, preactivation=None, input_gr
                                            _ptr(dx) if rows else None, _ptr(dw), _ptr(db), _ptr(ws), need,
                                            stream_ptr(device)))
     return dx, dw, db
+
+
+def _check_attention(q, k, v, scale) -> float:
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        if x.dim() != 4:
+            raise ValueError(f"{name} must be [batch, length, heads, dim], got shape {tuple(x.shape)}")
+    B, _, H, D = q.shape
+    if k.shape != v.shape:
+        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch and dim")
+    if H < 1 or k.shape[2] < 1 or H % k.shape[2]:
+        raise ValueError(f"the number of query heads ({H}) must be a multiple of the number of key heads ({k.shape[2]})")
+    if D < 1:
+        raise ValueError("dim must be positive")
+    if D > 128:
+        raise NotImplementedError(f"head dimensions beyond 128 are not supported (got {D})")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    return scale
+
+
+def _check_lengths(lengths, batch: int, keys: int):
+    """key_lengths as an int32 tensor (host or device); host values are checked."""
+    if lengths is None:
+        return None
+    if not isinstance(lengths, torch.Tensor):
+        lengths = torch.as_tensor(np.asarray(lengths))
+    if lengths.shape != (batch,) or lengths.dtype.is_floating_point or lengths.dtype in (torch.bool, torch.complex64):
+        raise ValueError(f"key_lengths must be {batch} integers, got {lengths.dtype} {tuple(lengths.shape)}")
+    if not lengths.is_cuda and batch and not 0 <= int(lengths.min()) <= int(lengths.max()) <= keys:
+        raise ValueError(f"key_lengths must lie in 0 .. {keys}")
+    if lengths.dtype != torch.int32:
+        lengths = lengths.clamp(0, keys).to(torch.int32)
+    return lengths.contiguous()
+
+
+def _heads(x: torch.Tensor) -> torch.Tensor:
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _strides(x: torch.Tensor):
+    return (ctypes.c_int64 * 3)(*x.stride()[:3])
+
+
+def _attention_desc(q, k, v, causal, scale) -> _lib.AttentionDesc:
+    return _lib.AttentionDesc(_DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3],
+                              int(bool(causal)), scale, _strides(q), _strides(k), _strides(v))
+
+
+def attention(q, k, v, causal: bool = False, key_lengths=None, scale=None, return_lse: bool = False):
+    """softmax(scale q k^T) v for every batch item and head.
+
+    q [B, Sq, H, D], k and v [B, Sk, Hk, D] of one type, D <= 128, H a multiple of Hk (query head h
+    uses key head h // (H // Hk)); any strides with D contiguous, so heads may be slices of one
+    projection's rows.  scale defaults to 1 / sqrt(D).  key_lengths [B]: keys at and behind an item's
+    length are neither seen nor read (padding may hold anything); values are brought into 0 .. Sk.
+    causal: query i sees keys j <= i + Sk - Sq.  A query that sees no key gets zeros.  A value that
+    is not finite in a key or value row which some query of a causal call sees may reach other
+    queries.
+
+    Returns out [B, Sq, H, D], contiguous; with return_lse also the logarithm of each row's sum of
+    exponentials, float32 [B, H, Sq] (-inf where no key is seen), which `attention_backward` takes.
+    Few queries over many keys (a decoding step) are split along the keys and joined.
+    """
+    ops = _operands(q=q, k=k, v=v)
+    _same_type(ops, ("q", "k", "v"))
+    scale = _check_attention(ops["q"], ops["k"], ops["v"], scale)
+    B, Sq, H, D = ops["q"].shape
+    ops["key_lengths"] = _check_lengths(key_lengths, B, ops["k"].shape[1])
+    device = _to_device(ops)
+    q, k, v = (_heads(ops[n]) for n in ("q", "k", "v"))
+    lengths = ops["key_lengths"]
+    out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=device)
+    lse = torch.empty((B, H, Sq), dtype=torch.float32, device=device) if return_lse else None
+    desc = _attention_desc(q, k, v, causal, scale)
+    lib = _lib.lib()
+    need = lib.mia_attention_workspace_bytes(ctypes.byref(desc))
+    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    with torch.cuda.device(device):
+        _lib.check(lib.mia_attention(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths),
+                                     out.data_ptr(), _ptr(lse), _ptr(ws), need, stream_ptr(device)))
+    return (out, lse) if return_lse else out
+
+
+def attention_backward(dout, q, k, v, out, lse, causal: bool = False, key_lengths=None, scale=None):
+    """Gradients (dq, dk, dv) of `attention` from its results `out` and `lse`.
+
+    dout and out [B, Sq, H, D], lse float32 [B, H, Sq]; the other arguments as in the forward call.
+    The probabilities are recomputed, nothing of size Sq x Sk is kept.  dk and dv are summed over the
+    query heads that share a key head, and zero behind a length.  For the products the
+    probabilities and their gradients are rounded to the operands' type.
+    """
+    ops = _operands(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
+    _same_type(ops, ("dout", "q", "k", "v", "out"))
+    scale = _check_attention(ops["q"], ops["k"], ops["v"], scale)
+    B, Sq, H, D = ops["q"].shape
+    for name in ("dout", "out"):
+        if ops[name].shape != ops["q"].shape:
+            raise ValueError(f"{name} must have q's shape {tuple(ops['q'].shape)}, got {tuple(ops[name].shape)}")
+    if ops["lse"].dtype != torch.float32 or ops["lse"].shape != (B, H, Sq):
+        raise ValueError(f"lse must be float32 of shape {(B, H, Sq)}, got {ops['lse'].dtype} {tuple(ops['lse'].shape)}")
+    ops["key_lengths"] = _check_lengths(key_lengths, B, ops["k"].shape[1])
+    device = _to_device(ops)
+    dout, q, k, v, out = (_heads(ops[n]) for n in ("dout", "q", "k", "v", "out"))
+    lse, lengths = ops["lse"].contiguous(), ops["key_lengths"]
+    dq = torch.empty((B, Sq, H, D), dtype=q.dtype, device=device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=device)
+    dv = torch.empty(k.shape, dtype=q.dtype, device=device)
+    desc = _attention_desc(q, k, v, causal, scale)
+    lib = _lib.lib()
+    need = lib.mia_attention_backward_workspace_bytes(ctypes.byref(desc))
+    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    with torch.cuda.device(device):
+        _lib.check(lib.mia_attention_backward(ctypes.byref(desc), dout.data_ptr(), _strides(dout), q.data_ptr(),
+                                              k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(out), lse.data_ptr(),
+                                              _ptr(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), need,
+                                              stream_ptr(device)))
+    return dq, dk, dv
