@@ -3,20 +3,25 @@
 
 namespace mia {
 // out[i] = sum of the groups' partial sums in order, in double
-__global__ __launch_bounds__(256) void lin_bias_join_kernel(const float* __restrict__ partial, int groups, int n,
+__global__ __launch_bounds__(1024) void lin_bias_join_kernel(const float* __restrict__ partial, int groups, int n,
                                                             float* __restrict__ out) {
-  __shared__ double part[4][64];
+  __shared__ double part[16][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int i = blockIdx.x * 64 + lane;
   double s = 0.0;
   if (i < n) {
-    const int per = (groups + 3) / 4;
+    const int per = (groups + 15) / 16;
     const int end = min(groups, (wv + 1) * per);
     for (int g = wv * per; g < end; ++g) s += (double)partial[(long long)g * n + i];
   }
   part[wv][lane] = s;
   __syncthreads();
-  if (wv == 0 && i < n) out[i] = (float)((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+  if (wv == 0 && i < n) {
+    s = 0.0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += part[k][lane];
+    out[i] = (float)s;
+  }
 }
 
 namespace lin {
@@ -118,7 +123,7 @@ int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_
       if (dz) g = dz, g_stride = out;
     }
     if (dbias) {
-      hipLaunchKernelGGL(lin_bias_join_kernel, dim3((unsigned)((out + 63) / 64)), dim3(256), 0, s, sums, groups,
+      hipLaunchKernelGGL(lin_bias_join_kernel, dim3((unsigned)((out + 63) / 64)), dim3(1024), 0, s, sums, groups,
                          (int)out, dbias);
     }
     lin::Epilogue e{nullptr, 0, MIA_ACT_NONE, nullptr, 0, nullptr, nullptr};

@@ -13,6 +13,7 @@
 #pragma once
 #include "nn_common.h"
 
+
 namespace mia {
 namespace lin {
 using namespace nn;
@@ -96,86 +97,84 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, int n) {
   return e.bias_f32 ? static_cast<const float*>(e.bias)[n] : (float)static_cast<const T*>(e.bias)[n];
 }
 
-// COUNT consecutive results of row m from column n0 on, `left` of them inside the row.
-template <class T, int COUNT>
-__device__ __forceinline__ void finish(const Epilogue& e, long long m, int n0, int left, int n, float* v) {
+// One 16-byte piece of results: V columns of a row from element `at` of out and z on, `left` of them
+// inside the row (>= V: all); b: the bias, r: the residual's piece.
+template <class T>
+__device__ __forceinline__ void finish(const Epilogue& e, long long at, int left, const float* b, u4 r, float* v) {
   constexpr int V = kPer16<T>;
   constexpr bool PRECISE = sizeof(T) == 4;
-  if (e.bias) {
-    if (left >= COUNT) {
-      float b[COUNT];
-      if (e.bias_f32) {
 #pragma unroll
-        for (int j = 0; j < COUNT; j += 4) unpack<float>(load_piece(static_cast<const float*>(e.bias) + n0 + j, 4), b + j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < COUNT; j += V) unpack<T>(load_piece(static_cast<const T*>(e.bias) + n0 + j, V), b + j);
-      }
-#pragma unroll
-      for (int j = 0; j < COUNT; ++j) v[j] += b[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < COUNT; ++j)
-        if (j < left) v[j] += bias_at<T>(e, n0 + j);
-    }
-  }
-  const long long at = m * n + n0;
-  if (e.z) {
-    T* z = static_cast<T*>(e.z) + at;
-#pragma unroll
-    for (int j = 0; j < COUNT; j += V) store_piece(z + j, pack<T>(v + j), left - j);
-  }
+  for (int j = 0; j < V; ++j) v[j] += b[j];
+  if (e.z) store_piece(static_cast<T*>(e.z) + at, pack<T>(v), left);
   if (e.act != MIA_ACT_NONE) {
 #pragma unroll
-    for (int j = 0; j < COUNT; ++j) v[j] = activate<PRECISE>(v[j], e.act);
+    for (int j = 0; j < V; ++j) v[j] = activate<PRECISE>(v[j], e.act);
   }
   if (e.residual) {
-    const T* r = static_cast<const T*>(e.residual) + m * e.residual_stride + n0;
-    float x[COUNT];
+    float x[V];
+    unpack<T>(r, x);
 #pragma unroll
-    for (int j = 0; j < COUNT; j += V) unpack<T>(load_piece(r + j, left - j), x + j);
-#pragma unroll
-    for (int j = 0; j < COUNT; ++j) v[j] += x[j];
+    for (int j = 0; j < V; ++j) v[j] += x[j];
   }
-  T* out = static_cast<T*>(e.out) + at;
+  store_piece(static_cast<T*>(e.out) + at, pack<T>(v), left);
+}
+// the bias of V columns from n on, zeros where there is none
+template <class T>
+__device__ __forceinline__ void load_bias(const Epilogue& e, int n, int left, float* b) {
+  constexpr int V = kPer16<T>;
 #pragma unroll
-  for (int j = 0; j < COUNT; j += V) store_piece(out + j, pack<T>(v + j), left - j);
+  for (int j = 0; j < V; ++j) b[j] = 0.0f;
+  if (!e.bias) return;
+  if (e.bias_f32) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) unpack<float>(load_piece(static_cast<const float*>(e.bias) + n + j, left - j), b + j);
+  } else {
+    unpack<T>(load_piece(static_cast<const T*>(e.bias) + n, left), b);
+  }
+}
+template <class T>
+__device__ __forceinline__ u4 load_residual(const Epilogue& e, long long m, int n, int left) {
+  if (!e.residual) return u4{0, 0, 0, 0};
+  return load_piece(static_cast<const T*>(e.residual) + m * e.residual_stride + n, left);
 }
 
 // 64 bytes that read as zero: the source of every piece that lies outside its operand.
 __device__ const u4 kZeros[4] = {};
 }  // namespace lin
 
-// Tile of BN x BM results, WN x WM waves.  An LDS stage holds 64 bytes of k of both operands.
-template <int BN_, int BM_, int WN_, int WM_, int STAGES_, int OCC_>
+// Tile of BN x BM results, WN x WM waves.  An LDS stage holds 128 bytes of k (two matrix steps) of both
+// operands: whole cache lines of an operand whose k is contiguous; two stages.
+template <int BN_, int BM_, int WN_, int WM_, int OCC_>
 struct LinTile {
-  static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, STAGES = STAGES_, OCC = OCC_;
+  static constexpr int BN = BN_, BM = BM_, WN = WN_, WM = WM_, OCC = OCC_;
   static constexpr int NW = WN * WM, WG = 64 * NW;
   static constexpr int TN = BN / WN, TM = BM / WM;  // a wave's part
   static constexpr int RN = TN / 16, RM = TM / 16;  // ... in accumulators of 16 x 16
-  static constexpr int A_BYTES = BN * 64, B_BYTES = BM * 64, STAGE = A_BYTES + B_BYTES;
-  static constexpr int PA = BN / (16 * NW), PB = BM / (16 * NW);  // 1 KiB pieces per wave and stage
-  static constexpr int LDS = STAGES * STAGE;
-  static_assert(TN % 64 == 0 && TM % 16 == 0 && BN % (16 * NW) == 0 && BM % (16 * NW) == 0, "whole pieces");
-  static_assert(LDS <= 160 * 1024, "LDS budget");
+  static constexpr int A_BYTES = BN * 128, B_BYTES = BM * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int PA = BN / (8 * NW), PB = BM / (8 * NW);  // 1 KiB pieces per wave and stage
+  static constexpr int LDS = 2 * STAGE;
+  static_assert(TN % 32 == 0 && TM % 16 == 0 && BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "whole pieces");
+  static_assert(LDS <= 160 * 1024 && (STAGE & (STAGE - 1)) == 0, "LDS budget");
 };
-using LinTile256 = LinTile<256, 256, 2, 4, 4, 1>;
-using LinTile128 = LinTile<128, 128, 2, 2, 4, 2>;
-using LinTile64 = LinTile<64, 64, 1, 4, 4, 4>;
+using LinTile256 = LinTile<256, 256, 2, 4, 1>;
+using LinTile128 = LinTile<128, 128, 2, 2, 2>;
+using LinTile64 = LinTile<64, 64, 1, 4, 4>;
 
 namespace lin {
 // One operand's tile in LDS and its fragments.  KC: k contiguous, LDS rows are `ROWS` operand rows
-// of four 16-byte pieces of k; otherwise LDS rows are the stage's k, ROWS elements each.  Piece c of
+// of eight 16-byte pieces of k; otherwise LDS rows are the stage's k, ROWS elements each.  Piece c of
 // LDS row r sits at piece position c ^ swizzle(r), so that the lanes of one LDS read fall on
 // different banks; with LDS-DMA the same permutation is applied to the source addresses.
-template <class T, bool KC, int ROWS>
+template <class T, bool KC, int ROWS, int Q>
 struct Operand {
   static constexpr int ES = (int)sizeof(T), V = 16 / ES;
-  static constexpr int KSTEP = 64 / ES;                           // k of a stage
-  static constexpr int PITCH = KC ? 64 : ROWS * ES;               // bytes of an LDS row
+  static constexpr int KSTEP = 128 / ES;                          // k of a stage
+  static constexpr int PITCH = KC ? 128 : ROWS * ES;              // bytes of an LDS row
   static constexpr int PIECES = PITCH / 16;                       // pieces of an LDS row
   static __device__ __forceinline__ int swizzle(int r) {
-    if constexpr (KC) return (r ^ (r >> 2)) & 3;
+    // a fragment read takes one piece of rows r .. r + 15 (Q = 4) or of 8 q + (0 .. 3) (Q = 8): two
+    // rows lie in one span of all banks, the other three bits of the row choose the position
+    if constexpr (KC) return Q == 4 ? (r >> 1) & 7 : ((r >> 1) & 1) | ((r >> 2) & 6);
     // column reads touch rows r .. r + 3 (two-byte: of 8 groups of rows) at one column range
     return ES == 2 ? (((r & 3) | ((r >> 1) & 4)) << 1) & (PIECES - 1) : ((r & 15) << 1) & (PIECES - 1);
   }
@@ -188,18 +187,19 @@ struct Operand {
       row = c * V, k = r;
     }
   }
-  // The 16-byte fragment of tile row `row0 + perm(lane & 15)`, k piece lane >> 4.  perm spreads the
-  // 16 rows as 16 (r >> 2) + (r & 3): with four accumulators at row0 = base + 4 t, lane group g of
-  // the result holds the 16 consecutive rows base + 16 g ...  (PERM; else rows row0 + r).
-  template <bool PERM>
-  static __device__ __forceinline__ u4 fragment(const unsigned char* tile, int row0, int lane) {
+  // The 16-byte fragment of tile row row0 + Q (r >> 2) + (r & 3), r = lane & 15, k piece 4 sub + (lane >> 4).
+  // Q = 4: rows in order.  Q = 8 (two-byte types, first operand): the accumulators at row0 = base and
+  // base + 4 together give lane group g of the result the rows base + 8 g ... + 7, so that a store of
+  // 16 bytes a lane writes 64 consecutive bytes of 16 rows.  (Down the columns Q = 8 uses half of the
+  // LDS banks at a time; with Q = 4 and stores of 8 bytes the gradients took 2 - 8 % longer.)
+  static __device__ __forceinline__ u4 fragment(const unsigned char* tile, int row0, int sub, int lane) {
     const int r15 = lane & 15, g = lane >> 4;
     if constexpr (KC) {
-      const int row = row0 + (PERM ? 16 * (r15 >> 2) + (r15 & 3) : r15);
-      return *reinterpret_cast<const u4*>(tile + row * 64 + ((g ^ swizzle(row)) << 4));
+      const int row = row0 + Q * (r15 >> 2) + (r15 & 3);
+      return *reinterpret_cast<const u4*>(tile + row * 128 + (((4 * sub + g) ^ swizzle(row)) << 4));
     } else if constexpr (ES == 2) {
-      const int col = row0 + (PERM ? 16 : 4) * (r15 & 3);  // this lane's quad of columns
-      const int k0 = 8 * g + (r15 >> 2);
+      const int col = row0 + Q * (r15 & 3);  // this lane's quad of columns
+      const int k0 = 32 * sub + 8 * g + (r15 >> 2);
       const unsigned base = (unsigned)(unsigned long long)tile;
       const int c = (col * 2) >> 4, in = (col * 2) & 15;
       const s4 lo = lds_read_column4(base + k0 * PITCH + ((c ^ swizzle(k0)) << 4) + in);
@@ -211,12 +211,12 @@ struct Operand {
       x.h[0] = lo, x.h[1] = hi;
       return x.u;
     } else {
-      const int col = row0 + (PERM ? 16 * (r15 >> 2) + (r15 & 3) : r15);
+      const int col = row0 + r15;
       const int c = col >> 2, in = (col & 3) * 4;
       u4 x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int k = 4 * g + j;
+        const int k = 16 * sub + 4 * g + j;
         x[j] = *reinterpret_cast<const unsigned*>(tile + k * PITCH + ((c ^ swizzle(k)) << 4) + in);
       }
       return x;
@@ -232,8 +232,9 @@ template <class TL, class T, bool AKC, bool BKC, bool DMA>
 __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) {
   using namespace lin;
   constexpr int ES = (int)sizeof(T);
-  using OA = Operand<T, AKC, TL::BN>;
-  using OB = Operand<T, BKC, TL::BM>;
+  constexpr int HALF = kPer16<T> / 4;  // accumulators that make up 16 bytes of a lane
+  using OA = Operand<T, AKC, TL::BN, 4 * HALF>;
+  using OB = Operand<T, BKC, TL::BM, 4>;
   constexpr int KSTEP = OA::KSTEP;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -264,13 +265,15 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
     for (int j = 0; j < TL::RM; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int wn = (wv % TL::WN) * TL::TN, wm = (wv / TL::WN) * TL::TM;
-  auto compute = [&](const unsigned char* stage) {
-    u4 fa[TL::RN], fb[TL::RM];
+  u4 fa[TL::RN], fb[TL::RM];
+  auto read = [&](const unsigned char* stage, int sub) {
 #pragma unroll
-    for (int j = 0; j < TL::RM; ++j) fb[j] = OB::template fragment<false>(stage + TL::A_BYTES, wm + 16 * j, lane);
+    for (int j = 0; j < TL::RM; ++j) fb[j] = OB::fragment(stage + TL::A_BYTES, wm + 16 * j, sub, lane);
 #pragma unroll
     for (int i = 0; i < TL::RN; ++i)
-      fa[i] = OA::template fragment<true>(stage, wn + 64 * (i / 4) + 4 * (i % 4), lane);
+      fa[i] = OA::fragment(stage, wn + 16 * HALF * (i / HALF) + 4 * (i % HALF), sub, lane);
+  };
+  auto multiply = [&] {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < TL::RN; ++i)
@@ -280,49 +283,94 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
   };
 
   if constexpr (DMA) {
-    // A ring of STAGES stages: while one is multiplied, the next STAGES - 1 are on their way.
-    constexpr int P = TL::PA + TL::PB, AHEAD = TL::STAGES - 1;
-    const char* src[P];
+    constexpr int P = TL::PA + TL::PB;
+    // A piece's place is a uniform base that moves with k and a fixed offset per lane.  Rows outside the
+    // operand repeat the last one (their results are never stored); the last stage of a k that is not a
+    // whole number of stages takes zeros behind it.
+    unsigned offset[P];
     int at_k[P];
-    long long adv[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const bool isa = i < TL::PA;
+      const bool isa = i < TL::PA, kc = isa ? AKC : BKC;
       const int s = (isa ? TL::PA * wv + i : TL::PB * wv + i - TL::PA) * 64 + lane;
       int row, k;
       if (isa) OA::where(s, row, k);
       else OB::where(s, row, k);
-      row += isa ? n0 : m0;
-      const bool in = row < (isa ? p.n : p.m);
-      k += k_begin;
-      const bool kc = isa ? AKC : BKC;
+      row = min(row, (isa ? p.n - n0 : p.m - m0) - (kc ? 1 : OA::V));
       const long long ld = isa ? p.lda : p.ldb;
-      src[i] = static_cast<const char*>(isa ? p.a : p.b) + (kc ? row * ld + k : k * ld + row) * ES;
-      adv[i] = (kc ? (long long)KSTEP : KSTEP * ld) * ES;
-      at_k[i] = in ? k : p.k;  // a row outside never comes in
+      offset[i] = (unsigned)((kc ? row * ld + k : k * ld + row) * ES);
+      at_k[i] = k;
     }
+    const char* base_a = static_cast<const char*>(p.a) + (AKC ? n0 * p.lda + k_begin : k_begin * p.lda + n0) * ES;
+    const char* base_b = static_cast<const char*>(p.b) + (BKC ? m0 * p.ldb + k_begin : k_begin * p.ldb + m0) * ES;
+    const long long step_a = (AKC ? (long long)KSTEP : KSTEP * p.lda) * ES;
+    const long long step_b = (BKC ? (long long)KSTEP : KSTEP * p.ldb) * ES;
+    int left_k = k_end - k_begin;  // behind the next stage's first k
     const unsigned lds0 = (unsigned)(unsigned long long)(smem);
-    auto issue = [&](int step) {
-      const unsigned buf = lds0 + (unsigned)(step % TL::STAGES) * TL::STAGE;
+    const unsigned lds_a = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + (unsigned)(TL::PA * wv) * 1024u));
+    const unsigned lds_b = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + TL::A_BYTES + (unsigned)(TL::PB * wv) * 1024u));
+    unsigned slot = 0;  // the two stages: byte 0 and byte STAGE
+    auto issue = [&] {
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const unsigned dst = buf + (i < TL::PA ? (unsigned)(TL::PA * wv + i) * 1024u
-                                               : TL::A_BYTES + (unsigned)(TL::PB * wv + i - TL::PA) * 1024u);
-        const char* from = at_k[i] < k_end ? src[i] : reinterpret_cast<const char*>(kZeros);
-        dma16(from, (unsigned)__builtin_amdgcn_readfirstlane((int)dst));
-        src[i] += adv[i];
-        at_k[i] += KSTEP;
+        const bool isa = i < TL::PA;
+        const char* base = isa ? base_a : base_b;
+        const unsigned dst = slot + (isa ? lds_a + 1024u * i : lds_b + 1024u * (i - TL::PA));
+        if (left_k >= KSTEP) dma16(base, offset[i], dst);
+        else dma16(at_k[i] < left_k ? base + offset[i] : reinterpret_cast<const char*>(kZeros), dst);
       }
+      base_a += step_a, base_b += step_b;
+      left_k -= KSTEP;
+      slot ^= TL::STAGE;
     };
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) issue(s);
-    for (int s = 0; s < steps; ++s) {
-      // stage s has landed for this wave; the barrier makes that all waves, and no wave still reads
-      // the stage that the next loads go to
-      wait_loads<P*(AHEAD - 1)>();
+    if constexpr (TL::NW == 8) {
+      // Two waves share a SIMD.  The waves of the second half run one phase behind: while one wave of
+      // a SIMD reads its fragments, the other one multiplies, so that neither the LDS nor the matrix
+      // cores wait for the other.  Barriers keep the phases.  Of stage s, with both steps:
+      //   first half    read 0 | multiply 0 | read 1     | multiply 1 | read 0 of s + 1
+      //   second half          | read 0     | multiply 0 | read 1     | multiply 1
+      // Buffer s is free when the second half has done read 1; from there to the first half's next
+      // read of that buffer lie four phases, in which its next stage arrives.
+      const bool second = wv >= 4;
+      issue();
+      if (steps > 1) issue();
+      if (steps > 1) wait_loads<P>();
+      else wait_loads<0>();
       barrier_keep_loads();
-      issue(s + AHEAD);  // (past the end: zeros, so that the count of loads in flight stays the same)
-      compute(smem + (s % TL::STAGES) * TL::STAGE);
+      if (second) barrier_keep_loads();
+      for (int s = 0; s < steps; ++s) {
+        const unsigned char* stage = smem + (s & 1) * TL::STAGE;
+        if (!second && s > 0 && s + 1 < steps) issue();
+        read(stage, 0);
+        wait_loads<63>();
+        barrier_keep_loads();
+        multiply();
+        barrier_keep_loads();
+        read(stage, 1);
+        if (second) wait_loads<0>();
+        else wait_loads<63>();
+        barrier_keep_loads();
+        if (second && s + 2 < steps) issue();
+        multiply();
+        if (!second) wait_loads<0>();
+        barrier_keep_loads();
+      }
+      if (!second) barrier_keep_loads();
+    } else {
+      issue();
+      for (int s = 0; s < steps; ++s) {
+        // stage s has landed for this wave; the barrier makes that all waves, and no wave still reads
+        // the buffer that the next loads go to
+        const unsigned char* stage = smem + (s & 1) * TL::STAGE;
+        wait_loads<0>();
+        barrier_keep_loads();
+        if (s + 1 < steps) issue();
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          read(stage, sub);
+          multiply();
+        }
+      }
     }
     wait_loads<0>();
   } else {
@@ -361,32 +409,72 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
       }
       __syncthreads();  // this stage is written; every wave is done with the other one
       if (s + 1 < steps) fetch(s + 1);
-      compute(stage);
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        read(stage, sub);
+        multiply();
+      }
     }
   }
 
-  // acc[i][j][v]: column n0 + wn + 64 (i / 4) + 16 g + 4 (i % 4) + v of row m0 + wm + 16 j + (lane & 15)
+  // accumulators HALF i ...: columns n0 + wn + 16 HALF i + V g ... of row m0 + wm + 16 j + (lane & 15)
+  constexpr int V = kPer16<T>, NP = TL::RN / HALF;
   const int g = lane >> 4;
+  const int n_first = n0 + wn + V * g;
+  auto finish_tile = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;  // no edge of the result inside this tile
+    float bias[NP][V];
+    u4 res[NP];
+    auto left_of = [&](int i) { return WHOLE ? V : p.n - (n_first + 16 * HALF * i); };
+    // loads of a row's pieces go out together, and ahead of the stores of the row before
+    auto fetch = [&](int j) {
+      const long long m = m0 + wm + 16 * j + (lane & 15);
 #pragma unroll
-  for (int j = 0; j < TL::RM; ++j) {
-    const long long m = m0 + wm + 16 * j + (lane & 15);
-    if (m >= p.m) continue;
+      for (int i = 0; i < NP; ++i)
+        res[i] = load_residual<T>(p.e, m, n_first + 16 * HALF * i, WHOLE || m < p.m ? left_of(i) : 0);
+    };
 #pragma unroll
-    for (int i = 0; i < TL::RN; i += 4) {
-      const int n = n0 + wn + 16 * i + 16 * g;
-      const int left = p.n - n;
-      if (left <= 0) continue;
-      float v[16];
+    for (int i = 0; i < NP; ++i) load_bias<T>(p.e, n_first + 16 * HALF * i, left_of(i), bias[i]);
+    if (p.e.residual) fetch(0);
 #pragma unroll
-      for (int t = 0; t < 16; ++t) v[t] = acc[i + t / 4][j][t % 4];
-      if (p.splits > 1) {
-        float* out = p.partial + ((long long)split * p.m + m) * p.n + n;
+    for (int j = 0; j < TL::RM; ++j) {
+      const long long m = m0 + wm + 16 * j + (lane & 15);
+      u4 now[NP];
 #pragma unroll
-        for (int t = 0; t < 16; t += 4) store_piece(out + t, pack<float>(v + t), left - t);
-      } else {
-        finish<T, 16>(p.e, m, n, left, p.n, v);
+      for (int i = 0; i < NP; ++i) now[i] = res[i];
+      if (p.e.residual && j + 1 < TL::RM) fetch(j + 1);
+      if (!WHOLE && m >= p.m) continue;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (!WHOLE && left_of(i) <= 0) continue;
+        float v[V];
+#pragma unroll
+        for (int t = 0; t < V; ++t) v[t] = acc[HALF * i + t / 4][j][t % 4];
+        finish<T>(p.e, m * p.n + n_first + 16 * HALF * i, left_of(i), bias[i], now[i], v);
       }
     }
+  };
+  if (p.splits > 1) {
+#pragma unroll
+    for (int j = 0; j < TL::RM; ++j) {
+      const long long m = m0 + wm + 16 * j + (lane & 15);
+      if (m >= p.m) continue;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int n = n_first + 16 * HALF * i, left = p.n - n;
+        if (left <= 0) continue;
+        float v[V];
+#pragma unroll
+        for (int t = 0; t < V; ++t) v[t] = acc[HALF * i + t / 4][j][t % 4];
+        float* out = p.partial + ((long long)split * p.m + m) * p.n + n;
+#pragma unroll
+        for (int t = 0; t < V; t += 4) store_piece(out + t, pack<float>(v + t), left - t);
+      }
+    }
+  } else if (n0 + TL::BN <= p.n && m0 + TL::BM <= p.m) {
+    finish_tile(std::true_type());
+  } else {
+    finish_tile(std::false_type());
   }
 }
 
@@ -394,22 +482,27 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
 template <class T>
 __global__ __launch_bounds__(256) void lin_join_kernel(lin::Gemm p) {
   using namespace lin;
-  const int per_row = (p.n + 7) / 8;
+  constexpr int V = kPer16<T>;
+  const int per_row = (p.n + V - 1) / V;
   const long long total = (long long)p.m * per_row;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long m = i / per_row;
-    const int n = (int)(i - m * per_row) * 8;
+    const int n = (int)(i - m * per_row) * V;
     const int left = p.n - n;
-    float v[8] = {};
+    float b[V], v[V] = {};
+    load_bias<T>(p.e, n, left, b);
+    const u4 r = load_residual<T>(p.e, m, n, left);
     for (int s = 0; s < p.splits; ++s) {
       const float* src = p.partial + ((long long)s * p.m + m) * p.n + n;
-      float x[8];
-      unpack<float>(load_piece(src, left), x);
-      unpack<float>(load_piece(src + 4, left - 4), x + 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += x[j];
+      for (int t = 0; t < V; t += 4) {
+        float x[4];
+        unpack<float>(load_piece(src + t, left - t), x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[t + j] += x[j];
+      }
     }
-    finish<T, 8>(p.e, m, n, left, p.n, v);
+    finish<T>(p.e, m * p.n + n, left, b, r, v);
   }
 }
 
@@ -537,7 +630,7 @@ static long long tiles_of(long long n, long long m, int tile) {
 
 // The tile and the number of parts of k, from the sizes alone (the workspace size follows from it).
 static Choice choose(long long n, long long m, long long k, size_t es, bool dma) {
-  const int kstep = (int)(64 / es);
+  const int kstep = (int)(128 / es);
   const long long steps = (k + kstep - 1) / kstep;
   Choice c{64, 1, 0};
   if (dma && tiles_of(n, m, 256) >= kCus) c.tile = 256;
@@ -546,7 +639,7 @@ static Choice choose(long long n, long long m, long long k, size_t es, bool dma)
   const long long fill = c.tile == 256 ? kCus : c.tile == 128 ? 2 * kCus : 4 * kCus;
   long long splits = 1;
   if (tiles < fill) splits = fill / tiles;
-  if (splits > steps / 16) splits = steps / 16;
+  if (splits > steps / 8) splits = steps / 8;
   if (splits > 32) splits = 32;
   if (splits < 1) splits = 1;
   const long long per = steps ? (steps + splits - 1) / splits : 1;
@@ -564,7 +657,7 @@ static int launch(Gemm g, hipStream_t s) {
     set_error("product too large for one launch");
     return MIA_ERR_UNSUPPORTED;
   }
-  constexpr int lds = DMA ? TL::LDS : 2 * TL::STAGE;
+  constexpr int lds = TL::LDS;
   auto kern = lin_gemm_kernel<TL, T, AKC, BKC, DMA>;
   if constexpr (lds > 64 * 1024) {
     MIA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
@@ -588,17 +681,17 @@ static int gemm(const Operands& o, const Epilogue& e, void* workspace, bool dma,
   }
   if (rc != MIA_OK) return rc;
   if (c.splits > 1) {
-    const long long work = o.m * ((o.n + 7) / 8);
+    const long long work = o.m * ((o.n + kPer16<T> - 1) / kPer16<T>);
     const long long blocks = (work + 255) / 256;
     hipLaunchKernelGGL(lin_join_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, g);
   }
   return MIA_OK;
 }
 
-// 16-byte pieces that are aligned and never cross the operand's edge
+// 16-byte pieces that are aligned and never cross the operand's edge, 256 rows within 32 bits of offset
 static bool pieces_ok(const void* p, long long ld, long long contiguous, size_t es) {
   const long long v = (long long)(16 / es);
-  return aligned16(p) && ld % v == 0 && contiguous % v == 0;
+  return aligned16(p) && ld % v == 0 && contiguous % v == 0 && ld * (long long)es < (1LL << 24);
 }
 
 static size_t split_bytes(long long n, long long m, long long k, size_t es) {

@@ -128,6 +128,16 @@ __device__ __forceinline__ void dma16(const void* gptr, unsigned lds_byte_addr) 
       : "v"(gptr), "s"(lds_byte_addr)
       : "memory");
 }
+// the same from a uniform base and a lane's unsigned byte offset: no address arithmetic per lane
+__device__ __forceinline__ void dma16(const void* base, unsigned offset, unsigned lds_byte_addr) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %0"
+      :
+      : "s"(base), "v"(offset), "s"(lds_byte_addr)
+      : "memory", "m0");
+}
 // the same with 4 bytes a lane, at lds_byte_addr + 4 L
 __device__ __forceinline__ void dma4(const void* gptr, unsigned lds_byte_addr) {
   unsigned keep;
