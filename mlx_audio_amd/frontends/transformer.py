@@ -22,54 +22,74 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .._runtime import require_gpu, stream_ptr
+from .._runtime import require_gpu
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _ACTIVATIONS = {None: _lib.ACT_NONE, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH, "relu": _lib.ACT_RELU}
 
 
 def _operands(**given) -> dict:
-    """The given arrays as tensors of a supported type that need no gradient (None stays None)."""
+    """The given arrays as tensors of a supported type that need no gradient, without the absent ones."""
     out = {}
     for name, x in given.items():
-        if x is not None and not isinstance(x, torch.Tensor):
+        if x is None:
+            continue
+        if not isinstance(x, torch.Tensor):
             x = torch.as_tensor(np.asarray(x))
-        if x is not None:
-            if x.dtype not in _DTYPES:
-                raise ValueError(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
-            if x.requires_grad and torch.is_grad_enabled():
-                raise RuntimeError(f"{name} requires a gradient, which this function does not record: call the "
-                                   "*_backward function for it, under torch.no_grad()")
+        if x.dtype not in _DTYPES:
+            raise ValueError(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires a gradient, which this function does not record: call the "
+                               "*_backward function for it, under torch.no_grad()")
         out[name] = x
     return out
 
 
 def _same_type(ops: dict, names) -> torch.dtype:
-    kinds = {n: ops[n].dtype for n in names if ops[n] is not None}
-    if len(set(kinds.values())) != 1:
-        raise ValueError("expected one type, got " + ", ".join(f"{n} {t}" for n, t in kinds.items()))
-    return next(iter(kinds.values()))
+    dtype = ops[names[0]].dtype
+    for n in names:
+        if n in ops and ops[n].dtype != dtype:
+            raise ValueError("expected one type, got " + ", ".join(f"{n} {ops[n].dtype}" for n in names if n in ops))
+    return dtype
 
 
 def _to_device(ops: dict) -> torch.device:
     """Moves host tensors to the device of the others (the current one if all are host tensors)."""
-    require_gpu()
-    devices = {x.device for x in ops.values() if x is not None and x.is_cuda}
-    if len(devices) > 1:
-        raise ValueError(f"tensors on different devices: {sorted(str(d) for d in devices)}")
-    device = devices.pop() if devices else torch.device("cuda", torch.cuda.current_device())
+    device, host = None, []
     for name, x in ops.items():
-        if x is not None and x.device != device:
-            ops[name] = x.to(device)
+        if x.device.type != "cuda":
+            host.append(name)
+        elif device is None:
+            device = x.device
+        elif x.device != device:
+            raise ValueError(f"tensors on different devices: {device}, {x.device}")
+    if device is None:
+        require_gpu()
+        device = torch.device("cuda", torch.cuda.current_device())
+    for name in host:
+        ops[name] = ops[name].to(device)
     return device
+
+
+def _call(fn, device: torch.device, *args) -> None:
+    """Enqueues on the device's current stream (the last argument of every entry point)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _rows(x: torch.Tensor):
     """x as (tensor, rows, row stride): last axis contiguous, leading axes collapsed."""
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    dim = x.shape[-1]
+    if dim > 1 and x.stride(-1) != 1:
         x = x.contiguous()
-    x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty((math.prod(x.shape[:-1]), x.shape[-1]))
-    return x, x.shape[0], (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+    if x.dim() != 2:
+        x = x.reshape(-1, dim) if x.numel() else x.new_empty((math.prod(x.shape[:-1]), dim))
+    rows = x.shape[0]
+    return x, rows, (x.stride(0) if rows > 1 else dim)
 
 
 def _ptr(x):
@@ -102,12 +122,13 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool 
     `layer_norm_backward` takes.  One launch that reads x once.
     """
     ops = _operands(x=x, weight=weight, bias=bias)
-    _check_norm(ops["x"], ops["weight"], ops["bias"])
+    _check_norm(ops["x"], ops.get("weight"), ops.get("bias"))
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative (got {eps})")
     device = _to_device(ops)
-    x, w, b = ops["x"], ops["weight"], ops["bias"]
-    w, b = (None if v is None else v.contiguous() for v in (w, b))
+    x, w, b = ops["x"], ops.get("weight"), ops.get("bias")
+    w = None if w is None else w.contiguous()
+    b = None if b is None else b.contiguous()
     flat, rows, stride = _rows(x)
     y = torch.empty(x.shape, dtype=x.dtype, device=device)
     mean = rstd = None
@@ -115,11 +136,9 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool 
         mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
         rstd = torch.empty_like(mean)
     params = next((v for v in (w, b) if v is not None), flat)
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().mia_layer_norm(flat.data_ptr(), rows, x.shape[-1], stride, _DTYPES[x.dtype], _ptr(w),
-                                             _ptr(b), _DTYPES[params.dtype], float(eps), y.data_ptr(),
-                                             _ptr(mean) if rows else None, _ptr(rstd) if rows else None,
-                                             stream_ptr(device)))
+    _call(_lib.lib().mia_layer_norm, device, flat.data_ptr(), rows, x.shape[-1], stride, _DTYPES[x.dtype], _ptr(w),
+          _ptr(b), _DTYPES[params.dtype], float(eps), y.data_ptr(), _ptr(mean) if rows else None,
+          _ptr(rstd) if rows else None)
     return (y, mean, rstd) if return_stats else y
 
 
@@ -131,7 +150,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     dy summed over its rows).  The sums have a fixed order: two calls give the same bits.
     """
     ops = _operands(dy=dy, x=x, mean=mean, rstd=rstd, weight=weight)
-    dy, x, mean, rstd, weight = (ops[n] for n in ("dy", "x", "mean", "rstd", "weight"))
+    dy, x, weight = ops["dy"], ops["x"], ops.get("weight")
     _check_norm(x, weight, None)
     _same_type(ops, ("dy", "x"))
     if dy.shape != x.shape:
@@ -155,11 +174,9 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
         db = torch.empty_like(dw)
         need = lib.mia_layer_norm_backward_workspace_bytes(rows, dim)
         ws = torch.empty((need,), dtype=torch.uint8, device=device)
-    with torch.cuda.device(device):
-        _lib.check(lib.mia_layer_norm_backward(gflat.data_ptr(), gstride, flat.data_ptr(), stride, mean.data_ptr(),
-                                               rstd.data_ptr(), rows, dim, _DTYPES[x.dtype], _ptr(w),
-                                               _DTYPES[(flat if w is None else w).dtype], dx.data_ptr(), _ptr(dw),
-                                               _ptr(db), _ptr(ws), need, stream_ptr(device)))
+    _call(lib.mia_layer_norm_backward, device, gflat.data_ptr(), gstride, flat.data_ptr(), stride, mean.data_ptr(),
+          rstd.data_ptr(), rows, dim, _DTYPES[x.dtype], _ptr(w), _DTYPES[(flat if w is None else w).dtype],
+          dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), need)
     return dx, dw, db
 
 
@@ -182,7 +199,7 @@ def linear(x, weight, bias=None, activation=None, residual=None, return_preactiv
     float32 matrix instruction.
     """
     ops = _operands(x=x, weight=weight, bias=bias, residual=residual)
-    x, weight, bias, residual = (ops[n] for n in ("x", "weight", "bias", "residual"))
+    x, weight, bias, residual = ops["x"], ops["weight"], ops.get("bias"), ops.get("residual")
     _check_linear(x, weight, activation)
     dtype = _same_type(ops, ("x", "weight", "residual"))
     n, k = weight.shape
@@ -202,11 +219,9 @@ def linear(x, weight, bias=None, activation=None, residual=None, return_preactiv
     lib = _lib.lib()
     need = lib.mia_linear_workspace_bytes(rows, k, n, _DTYPES[dtype])
     ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    with torch.cuda.device(device):
-        _lib.check(lib.mia_linear(flat.data_ptr(), stride, w.data_ptr(), wstride, _ptr(b),
-                                  _DTYPES[(flat if b is None else b).dtype], _ptr(r), rstride,
-                                  _ACTIVATIONS[activation], rows, k, n, _DTYPES[dtype], y.data_ptr(), _ptr(z),
-                                  _ptr(ws), need, stream_ptr(device)))
+    _call(lib.mia_linear, device, flat.data_ptr(), stride, w.data_ptr(), wstride, _ptr(b),
+          _DTYPES[(flat if b is None else b).dtype], _ptr(r), rstride, _ACTIVATIONS[activation], rows, k, n,
+          _DTYPES[dtype], y.data_ptr(), _ptr(z), _ptr(ws), need)
     return (y, z) if return_preactivation else y
 
 
@@ -221,7 +236,7 @@ def linear_backward(dy, x, weight, activation=None, preactivation=None, input_gr
     products dz is rounded to the operands' type.
     """
     ops = _operands(dy=dy, x=x, weight=weight, preactivation=preactivation)
-    dy, x, weight, z = (ops[n] for n in ("dy", "x", "weight", "preactivation"))
+    dy, x, weight, z = ops["dy"], ops["x"], ops["weight"], ops.get("preactivation")
     _check_linear(x, weight, activation)
     dtype = _same_type(ops, ("dy", "x", "weight", "preactivation"))
     n, k = weight.shape
@@ -247,11 +262,9 @@ def linear_backward(dy, x, weight, activation=None, preactivation=None, input_gr
     act = _ACTIVATIONS[activation]
     need = lib.mia_linear_backward_workspace_bytes(rows, k, n, _DTYPES[dtype], act)
     ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    with torch.cuda.device(device):
-        _lib.check(lib.mia_linear_backward(g.data_ptr(), gstride, flat.data_ptr(), stride, w.data_ptr(), wstride,
-                                           _ptr(zf), zstride, act, rows, k, n, _DTYPES[dtype],
-                                           _ptr(dx) if rows else None, _ptr(dw), _ptr(db), _ptr(ws), need,
-                                           stream_ptr(device)))
+    _call(lib.mia_linear_backward, device, g.data_ptr(), gstride, flat.data_ptr(), stride, w.data_ptr(), wstride,
+          _ptr(zf), zstride, act, rows, k, n, _DTYPES[dtype], _ptr(dx) if rows else None, _ptr(dw), _ptr(db), _ptr(ws),
+          need)
     return dx, dw, db
 
 
@@ -278,8 +291,6 @@ def _check_attention(q, k, v, scale) -> float:
 
 def _check_lengths(lengths, batch: int, keys: int):
     """key_lengths as an int32 tensor (host or device); host values are checked."""
-    if lengths is None:
-        return None
     if not isinstance(lengths, torch.Tensor):
         lengths = torch.as_tensor(np.asarray(lengths))
     if lengths.shape != (batch,) or lengths.dtype.is_floating_point or lengths.dtype in (torch.bool, torch.complex64):
@@ -323,19 +334,19 @@ def attention(q, k, v, causal: bool = False, key_lengths=None, scale=None, retur
     _same_type(ops, ("q", "k", "v"))
     scale = _check_attention(ops["q"], ops["k"], ops["v"], scale)
     B, Sq, H, D = ops["q"].shape
-    ops["key_lengths"] = _check_lengths(key_lengths, B, ops["k"].shape[1])
+    if key_lengths is not None:
+        ops["key_lengths"] = _check_lengths(key_lengths, B, ops["k"].shape[1])
     device = _to_device(ops)
     q, k, v = (_heads(ops[n]) for n in ("q", "k", "v"))
-    lengths = ops["key_lengths"]
+    lengths = ops.get("key_lengths")
     out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=device)
     lse = torch.empty((B, H, Sq), dtype=torch.float32, device=device) if return_lse else None
     desc = _attention_desc(q, k, v, causal, scale)
     lib = _lib.lib()
     need = lib.mia_attention_workspace_bytes(ctypes.byref(desc))
     ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    with torch.cuda.device(device):
-        _lib.check(lib.mia_attention(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths),
-                                     out.data_ptr(), _ptr(lse), _ptr(ws), need, stream_ptr(device)))
+    _call(lib.mia_attention, device, ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths),
+          out.data_ptr(), _ptr(lse), _ptr(ws), need)
     return (out, lse) if return_lse else out
 
 
@@ -356,10 +367,11 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool = False, key_length
             raise ValueError(f"{name} must have q's shape {tuple(ops['q'].shape)}, got {tuple(ops[name].shape)}")
     if ops["lse"].dtype != torch.float32 or ops["lse"].shape != (B, H, Sq):
         raise ValueError(f"lse must be float32 of shape {(B, H, Sq)}, got {ops['lse'].dtype} {tuple(ops['lse'].shape)}")
-    ops["key_lengths"] = _check_lengths(key_lengths, B, ops["k"].shape[1])
+    if key_lengths is not None:
+        ops["key_lengths"] = _check_lengths(key_lengths, B, ops["k"].shape[1])
     device = _to_device(ops)
     dout, q, k, v, out = (_heads(ops[n]) for n in ("dout", "q", "k", "v", "out"))
-    lse, lengths = ops["lse"].contiguous(), ops["key_lengths"]
+    lse, lengths = ops["lse"].contiguous(), ops.get("key_lengths")
     dq = torch.empty((B, Sq, H, D), dtype=q.dtype, device=device)
     dk = torch.empty(k.shape, dtype=q.dtype, device=device)
     dv = torch.empty(k.shape, dtype=q.dtype, device=device)
@@ -367,9 +379,7 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool = False, key_length
     lib = _lib.lib()
     need = lib.mia_attention_backward_workspace_bytes(ctypes.byref(desc))
     ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    with torch.cuda.device(device):
-        _lib.check(lib.mia_attention_backward(ctypes.byref(desc), dout.data_ptr(), _strides(dout), q.data_ptr(),
-                                              k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(out), lse.data_ptr(),
-                                              _ptr(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), need,
-                                              stream_ptr(device)))
+    _call(lib.mia_attention_backward, device, ctypes.byref(desc), dout.data_ptr(), _strides(dout), q.data_ptr(),
+          k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(out), lse.data_ptr(), _ptr(lengths), dq.data_ptr(),
+          dk.data_ptr(), dv.data_ptr(), _ptr(ws), need)
     return dq, dk, dv
