@@ -112,27 +112,51 @@ __device__ __forceinline__ u4 to_operand(const f4* blocks) {
   }
 }
 
-// Loads tiles of stream rows; rows at or past `end` and elements past dim read as zero whatever
-// memory holds there.  DMA: straight into LDS (pieces aligned, dim a whole number of them); else
-// through registers.
+// Loads tiles of stream rows; rows at or past `end` read as zero whatever memory holds there, and so
+// do elements past dim through registers.  DMA: straight into LDS (pieces aligned, dim a whole
+// number of them); a place is then a uniform base plus a fixed offset per lane, and pieces past dim
+// repeat the row's first one: the other operand is zero there, or the result is never stored.
 template <class T, int DP, bool DMA>
 struct Loader {
   using S = Shape<T, DP>;
+  unsigned offset[S::PW];
   u4 held[DMA ? 1 : S::PW];
-  __device__ __forceinline__ void issue(const void* base, long long stride, int row0, int end, int dim, unsigned lds,
-                                        int wv, int lane) {
+  static __device__ __forceinline__ void where(int i, int wv, int lane, int& r, int& c) {
+    const int s = (S::PW * wv + i) * 64 + lane;
+    r = s / S::PIECES, c = (s % S::PIECES) ^ (r & 7);
+  }
+  __device__ __forceinline__ void init(long long stride, int dim, int wv, int lane) {
 #pragma unroll
     for (int i = 0; i < S::PW; ++i) {
-      const int s = (S::PW * wv + i) * 64 + lane;
-      const int r = s / S::PIECES, c = (s % S::PIECES) ^ (r & 7);
-      const int row = row0 + r;
-      const T* from = static_cast<const T*>(base) + (long long)row * stride + c * S::V;
-      if constexpr (DMA) {
-        const void* src = row < end && c * S::V < dim ? static_cast<const void*>(from) : static_cast<const void*>(kZeros);
-        dma16(src, (unsigned)__builtin_amdgcn_readfirstlane((int)(lds + (unsigned)(S::PW * wv + i) * 1024u)));
+      int r, c;
+      where(i, wv, lane, r, c);
+      offset[i] = (unsigned)((r * stride + (c * S::V < dim ? c * S::V : 0)) * S::ES);
+    }
+  }
+  __device__ __forceinline__ void issue(const void* base, long long stride, int row0, int end, int dim, unsigned lds,
+                                        int wv, int lane) {
+    const char* from = static_cast<const char*>(base) + (long long)row0 * stride * S::ES;
+    if constexpr (DMA) {
+      const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds + (unsigned)(S::PW * wv) * 1024u));
+      if (row0 + S::TILE <= end) {
+#pragma unroll
+        for (int i = 0; i < S::PW; ++i) dma16(from, offset[i], dst + 1024u * i);
       } else {
+#pragma unroll
+        for (int i = 0; i < S::PW; ++i) {
+          int r, c;
+          where(i, wv, lane, r, c);
+          dma16(row0 + r < end ? from + offset[i] : reinterpret_cast<const char*>(kZeros), dst + 1024u * i);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::PW; ++i) {
+        int r, c;
+        where(i, wv, lane, r, c);
         held[i] = u4{0, 0, 0, 0};
-        if (row < end && c * S::V < dim) held[i] = load_piece(from, dim - c * S::V);
+        if (row0 + r < end && c * S::V < dim)
+          held[i] = load_piece(reinterpret_cast<const T*>(from) + r * stride + c * S::V, dim - c * S::V);
       }
     }
   }
@@ -144,6 +168,8 @@ struct Loader {
     }
   }
 };
+// Keeps the compiler from doing a rare branch's selects always.
+__device__ __forceinline__ void rarely() { asm volatile(""); }
 
 // An own row's vector as the second operand: step cc, elements V (4 cc + (lane >> 4)) ...
 template <class T, int DP>
@@ -171,10 +197,23 @@ __device__ __forceinline__ void store_own(T* row, int dim, int lane, const f4 (&
   }
 }
 
-// Workgroups that share a batch item and head follow each other on one XCD.
-__device__ __forceinline__ unsigned xcd_order() {
-  const unsigned nb = gridDim.x, id = blockIdx.x, q8 = nb / 8, r8 = nb % 8, xcd = id % 8;
-  return (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + id / 8;
+// The workgroup's pair (of batch item and head) and its index among the pair's `per` workgroups.
+// Workgroups go to the eight XCDs in turn; all of a pair go to one XCD, whose L2 then holds its keys
+// and values, and the pairs go round the XCDs, so that items of different lengths spread evenly.
+// With few pairs (less than 64) that would leave XCDs without work: in order then.  False: none.
+static inline unsigned order_grid(long long pairs, long long per) {
+  return (unsigned)(pairs < 64 ? pairs * per : (pairs + 7) / 8 * 8 * per);
+}
+__device__ __forceinline__ bool order(unsigned pairs, unsigned per, unsigned& pair, unsigned& index) {
+  if (pairs < 64) {
+    pair = blockIdx.x / per;
+    index = blockIdx.x - pair * per;
+    return true;
+  }
+  const unsigned local = blockIdx.x >> 3, turn = local / per;
+  index = local - turn * per;
+  pair = turn * 8 + (blockIdx.x & 7);
+  return pair < pairs;
 }
 __device__ __forceinline__ int keys_of(const Args& p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.sk) : p.sk;
@@ -201,13 +240,13 @@ __global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
 
-  unsigned id = xcd_order();
-  const int split = (int)(id % (unsigned)p.splits);
-  id /= (unsigned)p.splits;
-  const int tile = (int)(id % (unsigned)p.own_tiles);
-  id /= (unsigned)p.own_tiles;
   const int hgs = p.heads / p.pack;
-  const int hg = (int)(id % (unsigned)hgs), b = (int)(id / (unsigned)hgs);
+  unsigned pair, index;
+  if (!order((unsigned)(p.batch * hgs), (unsigned)(p.own_tiles * p.splits), pair, index)) return;
+  const int split = (int)(index % (unsigned)p.splits);
+  // (causal: the last rows see most keys, so they start first)
+  const int at_tile = (int)(index / (unsigned)p.splits), tile = p.causal ? p.own_tiles - 1 - at_tile : at_tile;
+  const int hg = (int)(pair % (unsigned)hgs), b = (int)(pair / (unsigned)hgs);
   const int kvh = hg * p.pack / (p.heads / p.kv_heads);
   const int rows = p.sq * p.pack;
   const int row0 = tile * (64 * OT) + wv * (16 * OT);
@@ -243,10 +282,10 @@ __global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
   }
 
   f4 acc[S::DT][OT];
-  float mx[OT], sum[OT];
+  float ref[OT], sum[OT];
 #pragma unroll
   for (int o = 0; o < OT; ++o) {
-    mx[o] = -kInf, sum[o] = 0.0f;
+    ref[o] = -kInf, sum[o] = 0.0f;
 #pragma unroll
     for (int d = 0; d < S::DT; ++d) acc[d][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -255,6 +294,8 @@ __global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
   const T* vp = static_cast<const T*>(p.v.p) + b * p.v.b + kvh * p.v.h;
   const unsigned lds0 = (unsigned)(unsigned long long)smem;
   Loader<T, DP, DMA> lk, lv;
+  lk.init(p.k.s, p.dim, wv, lane);
+  lv.init(p.v.s, p.dim, wv, lane);
   const int tiles = k_end > k_begin ? (k_end - k_begin + S::TILE - 1) / S::TILE : 0;
   if (tiles) {
     lk.issue(kp, p.k.s, k_begin, k_end, p.dim, lds0, wv, lane);
@@ -289,6 +330,7 @@ __global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
         for (int o = 0; o < OT; ++o) s[kb][o] = Mma<T>::step(f, own[o][cc], s[kb][o]);
       }
     if (k0 + S::TILE > min(open, k_end)) {
+      rarely();
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -304,25 +346,29 @@ __global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = fmaxf(m, s[kb][o][i]);
-      m = fmaxf(mx[o], column_max(m));
-      const float ms = m == -kInf ? 0.0f : m * c;  // a row that has seen nothing yet: exp2(-inf) = 0
-      if (__any(m > mx[o])) {
-        const float alpha = exp2_fast(fmaf(mx[o], c, -ms));
-        mx[o] = m;
+      // The reference that exponents are taken against follows the running maximum only when that is
+      // more than 8 above it: p then stays below 2^8 (far from any type's limit; a sum's precision does
+      // not depend on it), and after the first tiles nothing is rescaled any more.
+      if (__any(m * c > ref[o] + 8.0f)) {
+        rarely();
+        const float top = fmaxf(ref[o], column_max(m) * c);
+        const float alpha = top == -kInf ? 1.0f : exp2_fast(ref[o] - top);  // nothing seen yet: 0 or nothing to do
+        ref[o] = top;
         sum[o] *= alpha;
 #pragma unroll
         for (int d = 0; d < S::DT; ++d) acc[d][o] *= alpha;
       }
-      float part = 0.0f;
+      const float minus = ref[o] == -kInf ? 0.0f : -ref[o];  // a row that has seen nothing: exp2(-inf) = 0
+      float part[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = exp2_fast(fmaf(s[kb][o][i], c, -ms));
+          const float e = exp2_fast(fmaf(s[kb][o][i], c, minus));
           s[kb][o][i] = e;
-          part += e;
+          part[i & 1] += e;
         }
-      sum[o] += part;
+      sum[o] += part[0] + part[1];
     }
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
@@ -355,14 +401,14 @@ __global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
       store_own<float>(p.partial + row * p.dim, p.dim, lane, acc, o, 1.0f);
       if (g == 0) {
         float* ml = p.partial + (long long)p.splits * n * p.dim + row * 2;
-        ml[0] = mx[o] * c;
+        ml[0] = ref[o];
         ml[1] = total;
       }
     } else {
       // an empty row (sum 0) is zero; a NaN in the sum stays one
       store_own<T>(static_cast<T*>(p.o0) + (((long long)b * p.sq + s) * p.heads + h) * p.dim, p.dim, lane, acc, o,
                    total == 0.0f ? 0.0f : 1.0f / total);
-      if (g == 0 && p.lse) p.lse[at] = total == 0.0f ? -kInf : fmaf(mx[o], p.scale, logf(total));
+      if (g == 0 && p.lse) p.lse[at] = total == 0.0f ? -kInf : fmaf(ref[o], kLn2, logf(total));
     }
   }
 }
@@ -442,10 +488,10 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   __shared__ __attribute__((aligned(16))) unsigned char smem[4 * S::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
-  unsigned id = xcd_order();
-  const int tile = (int)(id % (unsigned)p.own_tiles);
-  id /= (unsigned)p.own_tiles;
-  const int h = (int)(id % (unsigned)p.heads), b = (int)(id / (unsigned)p.heads);
+  unsigned pair, index;
+  if (!order((unsigned)(p.batch * p.heads), (unsigned)p.own_tiles, pair, index)) return;
+  const int tile = p.causal ? p.own_tiles - 1 - (int)index : (int)index;
+  const int h = (int)(pair % (unsigned)p.heads), b = (int)(pair / (unsigned)p.heads);
   const int kvh = h / (p.heads / p.kv_heads);
   const int row0 = tile * (64 * OT) + wv * (16 * OT);
   const int off = p.sk - p.sq;
@@ -480,6 +526,8 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   const T* vp = static_cast<const T*>(p.v.p) + b * p.v.b + kvh * p.v.h;
   const unsigned lds0 = (unsigned)(unsigned long long)smem;
   Loader<T, DP, DMA> lk, lv;
+  lk.init(p.k.s, p.dim, wv, lane);
+  lv.init(p.v.s, p.dim, wv, lane);
   const int tiles = k_end > 0 ? (k_end + S::TILE - 1) / S::TILE : 0;
   if (tiles) {
     lk.issue(kp, p.k.s, 0, k_end, p.dim, lds0, wv, lane);
@@ -519,6 +567,16 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
             dp[r][o] = Mma<T>::step(fv, og[o][cc], dp[r][o]);
           }
         }
+      if (masked) {
+        rarely();
+#pragma unroll
+        for (int o = 0; o < OT; ++o)
+#pragma unroll
+          for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[r][o][i] = k0 + 16 * (st * S::RB + r) + 4 * g + i < limit[o] ? s[r][o][i] : -kInf;
+      }
       u4 df[OT];
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
@@ -527,9 +585,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
         for (int r = 0; r < S::RB; ++r)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float e = exp2_fast(fmaf(s[r][o][i], c, -lse2[o]));
-            if (masked) e = k0 + 16 * (st * S::RB + r) + 4 * g + i < limit[o] ? e : 0.0f;
-            blocks[r][i] = e * (dp[r][o][i] - delta[o]);
+            blocks[r][i] = exp2_fast(fmaf(s[r][o][i], c, -lse2[o])) * (dp[r][o][i] - delta[o]);
           }
         df[o] = to_operand<T>(blocks);
       }
@@ -559,10 +615,10 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   __shared__ float rows_lse[2][64], rows_delta[2][64];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
-  unsigned id = xcd_order();
-  const int tile = (int)(id % (unsigned)p.own_tiles);
-  id /= (unsigned)p.own_tiles;
-  const int kvh = (int)(id % (unsigned)p.kv_heads), b = (int)(id / (unsigned)p.kv_heads);
+  unsigned pair, index;
+  if (!order((unsigned)(p.batch * p.kv_heads), (unsigned)p.own_tiles, pair, index)) return;
+  const int tile = (int)index;  // (causal: the first keys are seen by most queries)
+  const int kvh = (int)(pair % (unsigned)p.kv_heads), b = (int)(pair / (unsigned)p.kv_heads);
   const int group = p.heads / p.kv_heads;
   const int key0 = tile * (64 * OT), row0 = key0 + wv * (16 * OT);
   const int off = p.sk - p.sq;
@@ -591,6 +647,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   const unsigned lse_at = (unsigned)(unsigned long long)&rows_lse[0][0];
   const unsigned delta_at = (unsigned)(unsigned long long)&rows_delta[0][0];
   Loader<T, DP, DMA> lq, lg;
+  lq.init(p.q.s, p.dim, wv, lane);
+  lg.init(p.dout.s, p.dim, wv, lane);
   auto issue = [&](int t) {
     const int h = kvh * group + t / per_head, q0 = first + t % per_head * S::TILE;
     const unsigned at = lds0 + (t & 1) * 2 * S::BYTES;
@@ -614,7 +672,6 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     const int q0 = first + t % per_head * S::TILE;
     if (t + 1 < tiles) issue(t + 1);
     if (row0 >= len) continue;
-    // rows of this tile at or past `open` see all of the wave's keys
     const bool masked = row0 + 16 * OT > len || (p.causal && row0 + 16 * OT - 1 > q0 + off);
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
@@ -642,20 +699,29 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
         lse2[r] = *reinterpret_cast<const f4*>(&rows_lse[t & 1][at]);
         delta[r] = *reinterpret_cast<const f4*>(&rows_delta[t & 1][at]);
       }
+      if (masked) {
+        rarely();
+#pragma unroll
+        for (int o = 0; o < OT; ++o) {
+          const int key = row0 + 16 * o + (lane & 15);
+#pragma unroll
+          for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int q = q0 + 16 * (st * S::RB + r) + 4 * g + i;
+              s[r][o][i] = key < len && (!p.causal || key <= q + off) ? s[r][o][i] : -kInf;
+            }
+        }
+      }
       u4 pf[OT], df[OT];
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
         f4 pb[S::RB], db[S::RB];
-        const int key = row0 + 16 * o + (lane & 15);
 #pragma unroll
         for (int r = 0; r < S::RB; ++r)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float e = exp2_fast(fmaf(s[r][o][i], c, -lse2[r][i]));
-            if (masked) {
-              const int q = q0 + 16 * (st * S::RB + r) + 4 * g + i;
-              e = key < len && (!p.causal || key <= q + off) ? e : 0.0f;
-            }
+            const float e = exp2_fast(fmaf(s[r][o][i], c, -lse2[r][i]));
             pb[r][i] = e;
             db[r][i] = e * (dp[r][o][i] - delta[r][i]);
           }
@@ -721,9 +787,10 @@ struct Ops {
   static int backward(Args a, const float* lse, float* stats, void* dq, void* dk, void* dv, hipStream_t s);
 };
 #ifdef MIA_ATTENTION_TYPE
+// 16-byte pieces are aligned, a tile's rows lie within 32 bits of offset
 static bool pieces_ok(const View& v, size_t es) {
   const long long n = (long long)(16 / es);
-  return aligned16(v.p) && v.b % n == 0 && v.s % n == 0 && v.h % n == 0;
+  return aligned16(v.p) && v.b % n == 0 && v.s % n == 0 && v.h % n == 0 && v.s * (long long)es < (1LL << 25);
 }
 #define MIA_ATT_LAUNCH(kernel, ot, grid)                                                                           \
   do {                                                                                                             \
@@ -746,13 +813,9 @@ template <class T>
 int Ops<T>::forward(Args a, hipStream_t s) {
   const Plan pl = plan_forward(a.batch, a.sq, a.sk, a.heads, a.kv_heads);
   a.pack = pl.pack, a.own_tiles = pl.own_tiles, a.splits = pl.splits, a.keys_per_split = pl.keys_per_split;
-  const long long grid = (long long)a.batch * (a.heads / a.pack) * a.own_tiles * a.splits;
-  if (grid >= (1LL << 31)) {
-    set_error("too many workgroups for one launch");
-    return MIA_ERR_UNSUPPORTED;
-  }
+  const unsigned grid = order_grid((long long)a.batch * (a.heads / a.pack), (long long)a.own_tiles * a.splits);
   const bool dma = a.dim % (16 / (int)sizeof(T)) == 0 && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T));
-  with_dma(dma, [&](auto dma) { MIA_ATT_LAUNCH(att_fwd_kernel, pl.own_blocks, (unsigned)grid); });
+  with_dma(dma, [&](auto dma) { MIA_ATT_LAUNCH(att_fwd_kernel, pl.own_blocks, grid); });
   if (a.splits > 1) {
     const long long rows = (long long)a.batch * a.heads * a.sq;
     hipLaunchKernelGGL(att_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
@@ -770,7 +833,7 @@ int Ops<T>::backward(Args a, const float* lse, float* stats, void* dq, void* dk,
     const int ot = a.dim * (int)sizeof(T) <= 128 ? own_blocks((long long)a.batch * a.kv_heads, a.sk) : 1;
     a.own_tiles = (a.sk + 64 * ot - 1) / (64 * ot);
     a.o0 = dk, a.o1 = dv;
-    const unsigned grid = (unsigned)a.batch * (unsigned)a.kv_heads * (unsigned)a.own_tiles;
+    const unsigned grid = order_grid((long long)a.batch * a.kv_heads, a.own_tiles);
     with_dma(whole && pieces_ok(a.q, sizeof(T)) && pieces_ok(a.dout, sizeof(T)),
              [&](auto dma) {
                if (ot == 2) hipLaunchKernelGGL((att_dkv_kernel<T, 64, 2, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);
@@ -782,7 +845,7 @@ int Ops<T>::backward(Args a, const float* lse, float* stats, void* dq, void* dk,
     const int ot = own_blocks((long long)a.batch * a.heads, a.sq);
     a.own_tiles = (a.sq + 64 * ot - 1) / (64 * ot);
     a.o0 = dq, a.o1 = nullptr;
-    const unsigned grid = (unsigned)a.batch * (unsigned)a.heads * (unsigned)a.own_tiles;
+    const unsigned grid = order_grid((long long)a.batch * a.heads, a.own_tiles);
     with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)),
              [&](auto dma) { MIA_ATT_LAUNCH(att_dq_kernel, ot, grid); });
   }
