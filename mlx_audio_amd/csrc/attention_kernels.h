@@ -63,25 +63,32 @@ struct Shape {
   static constexpr int PW = BYTES / 4096;          // 1 KiB pieces per wave and tile
 };
 
-// Piece c of row r lies at position c ^ (r & 7): rows read side by side fall on different banks.
+// Piece c of LDS row r lies at position c ^ turn(r), so that neither kind of read meets itself on a
+// bank: one piece of 16 rows (turn differs for rows that start on the same banks), or 32 bytes of
+// each of 8 rows down the columns (turn / 2 differs too; float: 64 bytes of every fourth row, turn / 4).
+template <class T, int DP>
+__device__ __forceinline__ int turn(int r) {
+  if (sizeof(T) == 4) return r & 15;
+  if (DP == 64) return (r & 6) | ((r >> 3) & 1);
+  return ((r & 7) << 1) | ((r >> 3) & 1);
+}
 // 16 bytes of 16 rows: row block `rb`, piece 4 cc + (lane >> 4)
 template <class T, int DP>
 __device__ __forceinline__ u4 rows_fragment(const unsigned char* tile, int rb, int cc, int lane) {
   using S = Shape<T, DP>;
   const int row = 16 * rb + (lane & 15), c = 4 * cc + (lane >> 4);
-  return *reinterpret_cast<const u4*>(tile + row * S::PITCH + ((c ^ (row & 7)) << 4));
+  return *reinterpret_cast<const u4*>(tile + row * S::PITCH + ((c ^ turn<T, DP>(row)) << 4));
 }
-// Columns: lane's column is d = 64 (dt / 4) + 16 (r >> 2) + 4 (dt % 4) + (r & 3), r = lane & 15 (so that
-// four accumulators of a lane group hold 16 consecutive d), its elements are the stream rows of step
-// `st` in the order of the product tiles: rows 4 (lane >> 4) + i of each 16-row block.
+// Columns: lane's column is d = 16 dt + (lane & 15), its elements are the stream rows of step `st` in
+// the order of the product tiles: rows 4 (lane >> 4) + i of each 16-row block.
 template <class T, int DP>
 __device__ __forceinline__ u4 columns_fragment(const unsigned char* tile, int st, int dt, int lane) {
   using S = Shape<T, DP>;
   const int r = lane & 15, g = lane >> 4;
   if constexpr (S::ES == 2) {
-    const int row = 32 * st + 4 * g + (r >> 2);
-    const int d = 64 * (dt >> 2) + 16 * (r & 3) + 4 * (dt & 3);
-    const unsigned at = (unsigned)(unsigned long long)tile + row * S::PITCH + (((d >> 3) ^ (row & 7)) << 4) + (d & 7) * 2;
+    const int row = 32 * st + 4 * g + (r >> 2), d = 16 * dt + 4 * (r & 3);
+    const unsigned at =
+        (unsigned)(unsigned long long)tile + row * S::PITCH + (((d >> 3) ^ turn<T, DP>(row)) << 4) + (d & 7) * 2;
     union {
       s4 h[2];
       u4 u;
@@ -90,12 +97,12 @@ __device__ __forceinline__ u4 columns_fragment(const unsigned char* tile, int st
     x.h[1] = lds_read_column4(at + 16 * S::PITCH);
     return x.u;
   } else {
-    const int d = 64 * (dt >> 2) + 16 * (r >> 2) + 4 * (dt & 3) + (r & 3);
+    const int d = 16 * dt + r;
     u4 x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * st + 4 * g + i;
-      x[i] = *reinterpret_cast<const unsigned*>(tile + row * S::PITCH + (((d >> 2) ^ (row & 7)) << 4) + (d & 3) * 4);
+      x[i] = *reinterpret_cast<const unsigned*>(tile + row * S::PITCH + (((d >> 2) ^ turn<T, DP>(row)) << 4) + (d & 3) * 4);
     }
     return x;
   }
@@ -123,7 +130,7 @@ struct Loader {
   u4 held[DMA ? 1 : S::PW];
   static __device__ __forceinline__ void where(int i, int wv, int lane, int& r, int& c) {
     const int s = (S::PW * wv + i) * 64 + lane;
-    r = s / S::PIECES, c = (s % S::PIECES) ^ (r & 7);
+    r = s / S::PIECES, c = (s % S::PIECES) ^ turn<T, DP>(r);
   }
   __device__ __forceinline__ void init(long long stride, int dim, int wv, int lane) {
 #pragma unroll
@@ -182,18 +189,25 @@ __device__ __forceinline__ void load_own(const T* row, bool in, int dim, int lan
     if (in && e < dim) out[cc] = load_piece(row + e, dim - e);
   }
 }
-// 16 consecutive values of a lane: accumulators 4 grp .. 4 grp + 3 of own column `c`
+// An own column's results: 4 consecutive d of every accumulator per lane.
 template <class T, int DT, int N>
 __device__ __forceinline__ void store_own(T* row, int dim, int lane, const f4 (&acc)[DT][N], int c, float factor) {
-  constexpr int V = kPer16<T>;
+  struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T e[4];
+  };
 #pragma unroll
-  for (int grp = 0; grp < DT / 4; ++grp) {
-    const int d = 64 * grp + 16 * (lane >> 4);
-    float v[16];
+  for (int dt = 0; dt < DT; ++dt) {
+    const int d = 16 * dt + 4 * (lane >> 4);
+    Four v;
 #pragma unroll
-    for (int t = 0; t < 16; ++t) v[t] = acc[4 * grp + t / 4][c][t % 4] * factor;
+    for (int i = 0; i < 4; ++i) v.e[i] = (T)(acc[dt][c][i] * factor);
+    if (d + 4 <= dim) {
+      *reinterpret_cast<Four*>(row + d) = v;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 16; j += V) store_piece(row + d + j, pack<T>(v + j), dim - d - j);
+      for (int i = 0; i < 3; ++i)
+        if (d + i < dim) row[d + i] = v.e[i];
+    }
   }
 }
 
