@@ -39,9 +39,10 @@ struct Args {
   int causal;         // query i sees keys <= i + sk - sq
   float scale;
   int own_tiles;      // workgroups along the own rows
-  int splits;         // forward: parts of the keys
+  int splits;         // parts of the stream rows (forward: of the keys)
   int keys_per_split;
-  float* partial;     // forward, splits > 1: (splits, rows, dim) sums, then (splits, rows, 2) max and sum
+  float* partial;     // forward, splits > 1: (splits, rows, dim) sums, then (splits, rows, 2) max and sum;
+                      // gradients: (splits, elements of dq) or (splits, elements of dk and of dv)
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -50,13 +51,15 @@ constexpr float kInf = __builtin_huge_valf();
 __device__ const u4 kZeros[1] = {};
 __device__ const float kInfinity[1] = {kInf};
 
+// DP: the head dimension rounded up to what is computed, a multiple of 32.
 template <class T, int DP>
 struct Shape {
   static constexpr int ES = (int)sizeof(T), V = 16 / ES;
   static constexpr int TILE = ES == 2 ? 64 : 32;   // stream rows of a tile
-  static constexpr int PITCH = DP * ES;            // bytes of an LDS row
+  static constexpr int WIDTH = DP <= 64 ? 64 : 128;  // elements of an LDS row
+  static constexpr int PITCH = WIDTH * ES;         // bytes of an LDS row
   static constexpr int PIECES = PITCH / 16;
-  static constexpr int CC = PITCH / 64;            // matrix steps along dim
+  static constexpr int CC = DP * ES / 64;          // matrix steps along dim
   static constexpr int DT = DP / 16;               // accumulators along dim
   static constexpr int RB = ES == 2 ? 2 : 1;       // 16-row blocks of one matrix step along stream rows
   static constexpr int BYTES = TILE * PITCH;
@@ -69,7 +72,7 @@ struct Shape {
 template <class T, int DP>
 __device__ __forceinline__ int turn(int r) {
   if (sizeof(T) == 4) return r & 15;
-  if (DP == 64) return (r & 6) | ((r >> 3) & 1);
+  if (DP <= 64) return (r & 6) | ((r >> 3) & 1);
   return ((r & 7) << 1) | ((r >> 3) & 1);
 }
 // 16 bytes of 16 rows: row block `rb`, piece 4 cc + (lane >> 4)
@@ -246,7 +249,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 // Forward.  OT: blocks of 16 queries per wave.
 template <class T, int DP, int OT, bool DMA>
-__global__ __launch_bounds__(256, 2) void att_fwd_kernel(att::Args p) {
+__global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_fwd_kernel(att::Args p) {
   using namespace att;
   using S = Shape<T, DP>;
   constexpr int KB = S::TILE / 16, STEPS = KB / S::RB;
@@ -503,8 +506,9 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
   unsigned pair, index;
-  if (!order((unsigned)(p.batch * p.heads), (unsigned)p.own_tiles, pair, index)) return;
-  const int tile = p.causal ? p.own_tiles - 1 - (int)index : (int)index;
+  if (!order((unsigned)(p.batch * p.heads), (unsigned)(p.own_tiles * p.splits), pair, index)) return;
+  const int split = (int)(index % (unsigned)p.splits), at_tile = (int)(index / (unsigned)p.splits);
+  const int tile = p.causal ? p.own_tiles - 1 - at_tile : at_tile;
   const int h = (int)(pair % (unsigned)p.heads), b = (int)(pair / (unsigned)p.heads);
   const int kvh = h / (p.heads / p.kv_heads);
   const int row0 = tile * (64 * OT) + wv * (16 * OT);
@@ -542,12 +546,14 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   Loader<T, DP, DMA> lk, lv;
   lk.init(p.k.s, p.dim, wv, lane);
   lv.init(p.v.s, p.dim, wv, lane);
-  const int tiles = k_end > 0 ? (k_end + S::TILE - 1) / S::TILE : 0;
-  if (tiles) {
-    lk.issue(kp, p.k.s, 0, k_end, p.dim, lds0, wv, lane);
-    lv.issue(vp, p.v.s, 0, k_end, p.dim, lds0 + S::BYTES, wv, lane);
+  const int all = k_end > 0 ? (k_end + S::TILE - 1) / S::TILE : 0;
+  const int begin = (int)((long long)all * split / p.splits), end = (int)((long long)all * (split + 1) / p.splits);
+  if (begin < end) {
+    const unsigned at = lds0 + (begin & 1) * 2 * S::BYTES;
+    lk.issue(kp, p.k.s, begin * S::TILE, k_end, p.dim, at, wv, lane);
+    lv.issue(vp, p.v.s, begin * S::TILE, k_end, p.dim, at + S::BYTES, wv, lane);
   }
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = begin; t < end; ++t) {
     unsigned char* kt = smem + (t & 1) * 2 * S::BYTES;
     unsigned char* vt = kt + S::BYTES;
     lk.commit(kt, wv, lane);
@@ -555,7 +561,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
     wait_loads<0>();
     barrier_keep_loads();
     const int k0 = t * S::TILE;
-    if (t + 1 < tiles) {
+    if (t + 1 < end) {
       const unsigned next = lds0 + ((t + 1) & 1) * 2 * S::BYTES;
       lk.issue(kp, p.k.s, k0 + S::TILE, k_end, p.dim, next, wv, lane);
       lv.issue(vp, p.v.s, k0 + S::TILE, k_end, p.dim, next + S::BYTES, wv, lane);
@@ -615,7 +621,9 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   for (int o = 0; o < OT; ++o) {
     const int s = row0 + 16 * o + (lane & 15);
     if (s >= p.sq) continue;
-    store_own<T>(static_cast<T*>(p.o0) + (((long long)b * p.sq + s) * p.heads + h) * p.dim, p.dim, lane, acc, o, p.scale);
+    const long long at = (((long long)b * p.sq + s) * p.heads + h) * p.dim;
+    if (p.splits > 1) store_own<float>(p.partial + split * n * p.dim + at, p.dim, lane, acc, o, p.scale);
+    else store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, acc, o, p.scale);
   }
 }
 
@@ -630,8 +638,9 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
   unsigned pair, index;
-  if (!order((unsigned)(p.batch * p.kv_heads), (unsigned)p.own_tiles, pair, index)) return;
-  const int tile = (int)index;  // (causal: the first keys are seen by most queries)
+  if (!order((unsigned)(p.batch * p.kv_heads), (unsigned)(p.own_tiles * p.splits), pair, index)) return;
+  const int split = (int)(index % (unsigned)p.splits);
+  const int tile = (int)(index / (unsigned)p.splits);  // (causal: the first keys are seen by most queries)
   const int kvh = (int)(pair % (unsigned)p.kv_heads), b = (int)(pair / (unsigned)p.kv_heads);
   const int group = p.heads / p.kv_heads;
   const int key0 = tile * (64 * OT), row0 = key0 + wv * (16 * OT);
@@ -655,7 +664,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   // the first query that sees any of these keys; a workgroup past the length has nothing to do
   const int first = p.causal ? max(0, key0 - off) / S::TILE * S::TILE : 0;
   const int per_head = key0 < len && first < p.sq ? (p.sq - first + S::TILE - 1) / S::TILE : 0;
-  const int tiles = per_head * group;
+  const int all = per_head * group;
+  const int begin = (int)((long long)all * split / p.splits), end = (int)((long long)all * (split + 1) / p.splits);
   const long long n = (long long)p.batch * p.heads * p.sq;
   const unsigned lds0 = (unsigned)(unsigned long long)smem;
   const unsigned lse_at = (unsigned)(unsigned long long)&rows_lse[0][0];
@@ -675,8 +685,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
       dma4(in ? from + n : reinterpret_cast<const float*>(kZeros),
            (unsigned)__builtin_amdgcn_readfirstlane((int)(delta_at + (t & 1) * 256u)));
   };
-  if (tiles) issue(0);
-  for (int t = 0; t < tiles; ++t) {
+  if (begin < end) issue(begin);
+  for (int t = begin; t < end; ++t) {
     unsigned char* qt = smem + (t & 1) * 2 * S::BYTES;
     unsigned char* gt = qt + S::BYTES;
     lq.commit(qt, wv, lane);
@@ -684,7 +694,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     wait_loads<0>();
     barrier_keep_loads();
     const int q0 = first + t % per_head * S::TILE;
-    if (t + 1 < tiles) issue(t + 1);
+    if (t + 1 < end) issue(t + 1);
     if (row0 >= len) continue;
     const bool masked = row0 + 16 * OT > len || (p.causal && row0 + 16 * OT - 1 > q0 + off);
 #pragma unroll
@@ -759,8 +769,25 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     const int s = row0 + 16 * o + (lane & 15);
     if (s >= p.sk) continue;
     const long long at = (((long long)b * p.sk + s) * p.kv_heads + kvh) * p.dim;
-    store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, dk, o, p.scale);
-    store_own<T>(static_cast<T*>(p.o1) + at, p.dim, lane, dv, o, 1.0f);
+    if (p.splits > 1) {
+      const long long count = (long long)p.batch * p.sk * p.kv_heads * p.dim;
+      store_own<float>(p.partial + 2 * split * count + at, p.dim, lane, dk, o, p.scale);
+      store_own<float>(p.partial + (2 * split + 1) * count + at, p.dim, lane, dv, o, 1.0f);
+    } else {
+      store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, dk, o, p.scale);
+      store_own<T>(static_cast<T*>(p.o1) + at, p.dim, lane, dv, o, 1.0f);
+    }
+  }
+}
+
+// A gradient's parts added in order: out[i] = sum over splits of partial[split * stride + i].
+template <class T>
+__global__ __launch_bounds__(256) void att_add_kernel(const float* __restrict__ partial, long long stride, int splits,
+                                                      long long n, T* __restrict__ out) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    float v = partial[i];
+    for (int s = 1; s < splits; ++s) v += partial[s * stride + i];
+    out[i] = (T)v;
   }
 }
 
@@ -793,7 +820,35 @@ static Plan plan_forward(long long batch, long long sq, long long sk, int heads,
   p.keys_per_split = (int)per;
   return p;
 }
-static int own_blocks(long long outer, long long rows) { return outer * ((rows + 127) / 128) >= 2 * kCus && rows > 64 ? 2 : 1; }
+// One gradient kernel: `outer` pairs of `own` rows each, `stream` tiles to run over per workgroup.
+struct GradPlan {
+  int own_blocks, own_tiles, splits;
+};
+static GradPlan plan_gradient(long long outer, long long own, long long stream, bool two_blocks) {
+  GradPlan p;
+  p.own_blocks = two_blocks && own > 64 && outer * ((own + 127) / 128) >= 2 * kCus ? 2 : 1;
+  p.own_tiles = (int)((own + 64 * p.own_blocks - 1) / (64 * p.own_blocks));
+  const long long groups = outer * p.own_tiles;
+  long long splits = groups ? 2 * kCus / groups : 1;  // two workgroups per compute unit
+  if (splits > stream / 4) splits = stream / 4;       // of at least four tiles each
+  if (splits > 16) splits = 16;
+  p.splits = splits < 1 ? 1 : (int)splits;
+  return p;
+}
+static long long stream_tiles(long long rows, size_t es) { return (rows + (es == 2 ? 63 : 31)) / (es == 2 ? 64 : 32); }
+static GradPlan plan_dkv(long long batch, long long sq, long long sk, int heads, int kv_heads, int dim, size_t es) {
+  // (two blocks of keys with vectors of more than 128 bytes would not fit the registers)
+  return plan_gradient(batch * kv_heads, sk, stream_tiles(sq, es) * (heads / kv_heads), dim * (int)es <= 128);
+}
+static GradPlan plan_dq(long long batch, long long sq, long long sk, int heads, size_t es) {
+  return plan_gradient(batch * heads, sq, stream_tiles(sk, es), true);
+}
+static size_t gradient_bytes(long long batch, long long sq, long long sk, int heads, int kv_heads, int dim, size_t es) {
+  const GradPlan k = plan_dkv(batch, sq, sk, heads, kv_heads, dim, es), q = plan_dq(batch, sq, sk, heads, es);
+  const size_t kb = k.splits > 1 ? (size_t)2 * k.splits * batch * sk * kv_heads * dim * sizeof(float) : 0;
+  const size_t qb = q.splits > 1 ? (size_t)q.splits * batch * sq * heads * dim * sizeof(float) : 0;
+  return align256((size_t)2 * batch * heads * sq * sizeof(float)) + (kb > qb ? kb : qb);
+}
 
 template <class T>
 struct Ops {
@@ -806,15 +861,14 @@ static bool pieces_ok(const View& v, size_t es) {
   const long long n = (long long)(16 / es);
   return aligned16(v.p) && v.b % n == 0 && v.s % n == 0 && v.h % n == 0 && v.s * (long long)es < (1LL << 25);
 }
-#define MIA_ATT_LAUNCH(kernel, ot, grid)                                                                           \
-  do {                                                                                                             \
-    if (a.dim <= 64) {                                                                                             \
-      if (ot == 2) hipLaunchKernelGGL((kernel<T, 64, 2, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);   \
-      else hipLaunchKernelGGL((kernel<T, 64, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);           \
-    } else {                                                                                                       \
-      if (ot == 2) hipLaunchKernelGGL((kernel<T, 128, 2, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);  \
-      else hipLaunchKernelGGL((kernel<T, 128, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);          \
-    }                                                                                                              \
+#define MIA_ATT_ONE(kernel, dp, ot, grid) \
+  hipLaunchKernelGGL((kernel<T, dp, ot, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a)
+#define MIA_ATT_LAUNCH(kernel, ot, grid)                 \
+  do {                                                   \
+    if (a.dim <= 32) MIA_ATT_ONE(kernel, 32, ot, grid);  \
+    else if (a.dim <= 64) MIA_ATT_ONE(kernel, 64, ot, grid); \
+    else if (a.dim <= 96) MIA_ATT_ONE(kernel, 96, ot, grid); \
+    else MIA_ATT_ONE(kernel, 128, ot, grid);             \
   } while (0)
 
 template <class F>
@@ -829,7 +883,10 @@ int Ops<T>::forward(Args a, hipStream_t s) {
   a.pack = pl.pack, a.own_tiles = pl.own_tiles, a.splits = pl.splits, a.keys_per_split = pl.keys_per_split;
   const unsigned grid = order_grid((long long)a.batch * (a.heads / a.pack), (long long)a.own_tiles * a.splits);
   const bool dma = a.dim % (16 / (int)sizeof(T)) == 0 && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T));
-  with_dma(dma, [&](auto dma) { MIA_ATT_LAUNCH(att_fwd_kernel, pl.own_blocks, grid); });
+  with_dma(dma, [&](auto dma) { 
+    if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_fwd_kernel, 2, grid);
+    else MIA_ATT_LAUNCH(att_fwd_kernel, 1, grid);
+  });
   if (a.splits > 1) {
     const long long rows = (long long)a.batch * a.heads * a.sq;
     hipLaunchKernelGGL(att_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
@@ -840,28 +897,47 @@ template <class T>
 int Ops<T>::backward(Args a, const float* lse, float* stats, void* dq, void* dk, void* dv, hipStream_t s) {
   const long long rows = (long long)a.batch * a.heads * a.sq;
   const bool whole = a.dim % (16 / (int)sizeof(T)) == 0;
-  a.stats = stats, a.splits = 1, a.pack = 1;
+  a.stats = stats, a.pack = 1;
+  a.partial = stats + align256((size_t)2 * rows * sizeof(float)) / sizeof(float);
   if (rows) hipLaunchKernelGGL(att_stats_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, lse, stats);
+  auto add = [&](const float* partial, long long stride, long long n, void* out) {
+    const long long blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, partial,
+                       stride, a.splits, n, static_cast<T*>(out));
+  };
   if (a.sk) {
-    // (two blocks of keys with vectors of 256 bytes and more would not fit the registers)
-    const int ot = a.dim * (int)sizeof(T) <= 128 ? own_blocks((long long)a.batch * a.kv_heads, a.sk) : 1;
-    a.own_tiles = (a.sk + 64 * ot - 1) / (64 * ot);
+    const GradPlan pl = plan_dkv(a.batch, a.sq, a.sk, a.heads, a.kv_heads, a.dim, sizeof(T));
+    a.own_tiles = pl.own_tiles, a.splits = pl.splits;
     a.o0 = dk, a.o1 = dv;
-    const unsigned grid = order_grid((long long)a.batch * a.kv_heads, a.own_tiles);
-    with_dma(whole && pieces_ok(a.q, sizeof(T)) && pieces_ok(a.dout, sizeof(T)),
-             [&](auto dma) {
-               if (ot == 2) hipLaunchKernelGGL((att_dkv_kernel<T, 64, 2, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);
-               else if (a.dim <= 64) hipLaunchKernelGGL((att_dkv_kernel<T, 64, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);
-               else hipLaunchKernelGGL((att_dkv_kernel<T, 128, 1, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a);
-             });
+    const unsigned grid = order_grid((long long)a.batch * a.kv_heads, (long long)a.own_tiles * a.splits);
+    with_dma(whole && pieces_ok(a.q, sizeof(T)) && pieces_ok(a.dout, sizeof(T)), [&](auto dma) {
+      if (pl.own_blocks == 2) {
+        if constexpr (sizeof(T) == 2) {
+          if (a.dim <= 32) MIA_ATT_ONE(att_dkv_kernel, 32, 2, grid);
+          else MIA_ATT_ONE(att_dkv_kernel, 64, 2, grid);
+        } else {
+          MIA_ATT_ONE(att_dkv_kernel, 32, 2, grid);
+        }
+      } else {
+        MIA_ATT_LAUNCH(att_dkv_kernel, 1, grid);
+      }
+    });
+    if (a.splits > 1) {
+      const long long n = (long long)a.batch * a.sk * a.kv_heads * a.dim;
+      add(a.partial, 2 * n, n, dk);
+      add(a.partial + n, 2 * n, n, dv);
+    }
   }
   if (rows) {
-    const int ot = own_blocks((long long)a.batch * a.heads, a.sq);
-    a.own_tiles = (a.sq + 64 * ot - 1) / (64 * ot);
+    const GradPlan pl = plan_dq(a.batch, a.sq, a.sk, a.heads, sizeof(T));
+    a.own_tiles = pl.own_tiles, a.splits = pl.splits;
     a.o0 = dq, a.o1 = nullptr;
-    const unsigned grid = order_grid((long long)a.batch * a.heads, a.own_tiles);
-    with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)),
-             [&](auto dma) { MIA_ATT_LAUNCH(att_dq_kernel, ot, grid); });
+    const unsigned grid = order_grid((long long)a.batch * a.heads, (long long)a.own_tiles * a.splits);
+    with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)), [&](auto dma) {
+      if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_dq_kernel, 2, grid);
+      else MIA_ATT_LAUNCH(att_dq_kernel, 1, grid);
+    });
+    if (a.splits > 1) add(a.partial, rows * a.dim, rows * a.dim, dq);
   }
   return MIA_OK;
 }

@@ -97,26 +97,37 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, int n) {
   return e.bias_f32 ? static_cast<const float*>(e.bias)[n] : (float)static_cast<const T*>(e.bias)[n];
 }
 
-// One 16-byte piece of results: V columns of a row from element `at` of out and z on, `left` of them
-// inside the row (>= V: all); b: the bias, r: the residual's piece.
-template <class T>
-__device__ __forceinline__ void finish(const Epilogue& e, long long at, int left, const float* b, u4 r, float* v) {
+// One 16-byte piece of results: V columns of a row from `out` and `z` on, `left` of them inside the row
+// (>= V: all); b: the bias, r: the residual's piece (zeros where there is none).
+template <class T, int ACT, bool PLUS>
+__device__ __forceinline__ void finish(T* out, T* z, int left, const float* b, u4 r, float* v) {
   constexpr int V = kPer16<T>;
   constexpr bool PRECISE = sizeof(T) == 4;
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] += b[j];
-  if (e.z) store_piece(static_cast<T*>(e.z) + at, pack<T>(v), left);
-  if (e.act != MIA_ACT_NONE) {
+  if (z) store_piece(z, pack<T>(v), left);
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = activate<PRECISE>(v[j], e.act);
-  }
-  if (e.residual) {
+  for (int j = 0; j < V; ++j) v[j] = activate<PRECISE>(v[j], ACT);
+  if constexpr (PLUS) {
     float x[V];
     unpack<T>(r, x);
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += x[j];
   }
-  store_piece(static_cast<T*>(e.out) + at, pack<T>(v), left);
+  store_piece(out, pack<T>(v), left);
+}
+// Calls f(activation, with or without residual) with what the epilogue asks for as constants: one
+// branch before the results instead of several at each of them.
+template <class F>
+__device__ __forceinline__ void with_epilogue(const Epilogue& e, F f) {
+  auto plus = [&](auto act) {
+    if (e.residual) f(act, std::true_type());
+    else f(act, std::false_type());
+  };
+  if (e.act == MIA_ACT_GELU) plus(std::integral_constant<int, MIA_ACT_GELU>());
+  else if (e.act == MIA_ACT_GELU_TANH) plus(std::integral_constant<int, MIA_ACT_GELU_TANH>());
+  else if (e.act == MIA_ACT_RELU) plus(std::integral_constant<int, MIA_ACT_RELU>());
+  else plus(std::integral_constant<int, MIA_ACT_NONE>());
 }
 // the bias of V columns from n on, zeros where there is none
 template <class T>
@@ -134,7 +145,6 @@ __device__ __forceinline__ void load_bias(const Epilogue& e, int n, int left, fl
 }
 template <class T>
 __device__ __forceinline__ u4 load_residual(const Epilogue& e, long long m, int n, int left) {
-  if (!e.residual) return u4{0, 0, 0, 0};
   return load_piece(static_cast<const T*>(e.residual) + m * e.residual_stride + n, left);
 }
 
@@ -225,239 +235,215 @@ struct Operand {
 };
 }  // namespace lin
 
-// DMA: every 16-byte piece of both operands is aligned (bases, row strides) and lies either wholly
-// inside its operand or wholly outside; otherwise pieces go through registers, element by element
-// at the edges.
-template <class TL, class T, bool AKC, bool BKC, bool DMA>
-__global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) {
-  using namespace lin;
-  constexpr int ES = (int)sizeof(T);
-  constexpr int HALF = kPer16<T> / 4;  // accumulators that make up 16 bytes of a lane
-  using OA = Operand<T, AKC, TL::BN, 4 * HALF>;
-  using OB = Operand<T, BKC, TL::BM, 4>;
-  constexpr int KSTEP = OA::KSTEP;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-  // Consecutive logical tiles go to one XCD (one L2).  Inside, columns of four tiles along m: the
-  // tiles in flight on an XCD share their rows of both operands.
-  const unsigned nb = gridDim.x, id = blockIdx.x;
-  const unsigned q8 = nb / 8, r8 = nb % 8, xcd = id % 8;
-  unsigned logical = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + id / 8;
+namespace lin {
+// One workgroup's piece of the product: a tile of the result and a range of k.
+struct Place {
+  int n0, m0, k_begin, k_end, split;
+};
+// `logical` counts tiles so that neighbours share rows of both operands: columns of four tiles along m.
+template <class TL>
+__device__ __forceinline__ Place place(const Gemm& p, unsigned logical) {
+  Place w;
   const unsigned tiles = (unsigned)p.n_tiles * (unsigned)p.m_tiles;
-  const unsigned split = logical / tiles;
-  logical -= split * tiles;
+  w.split = (int)(logical / tiles);
+  logical -= (unsigned)w.split * tiles;
   constexpr unsigned GM = 4;
   const unsigned group = logical / (GM * (unsigned)p.n_tiles);
   const unsigned in_group = logical - group * GM * (unsigned)p.n_tiles;
   const unsigned gm = min(GM, (unsigned)p.m_tiles - group * GM);
-  const int n0 = (int)(in_group / gm) * TL::BN;
-  const int m0 = (int)(group * GM + in_group % gm) * TL::BM;
-  const int k_begin = (int)split * p.k_per_split;
-  const int k_end = min(p.k, k_begin + p.k_per_split);
-  const int steps = (k_end - k_begin + KSTEP - 1) / KSTEP;
+  w.n0 = (int)(in_group / gm) * TL::BN;
+  w.m0 = (int)(group * GM + in_group % gm) * TL::BM;
+  w.k_begin = w.split * p.k_per_split;
+  w.k_end = min(p.k, w.k_begin + p.k_per_split);
+  return w;
+}
+// Workgroups go to the eight XCDs in turn: XCD x gets a contiguous share [first, first + count) of
+// `total` tiles, so that one L2 serves neighbours.
+__device__ __forceinline__ void xcd_share(unsigned total, unsigned xcd, unsigned& first, unsigned& count) {
+  const unsigned q = total / 8, r = total % 8;
+  first = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q;
+  count = q + (xcd < r ? 1 : 0);
+}
 
-  f4 acc[TL::RN][TL::RM];
-#pragma unroll
-  for (int i = 0; i < TL::RN; ++i)
-#pragma unroll
-    for (int j = 0; j < TL::RM; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+// The stream of LDS-DMA loads of one wave.  A piece's place is a uniform base that moves with k and a
+// fixed offset per lane.  Rows outside the operand repeat the last one (their results are never
+// stored); the last stage of a k that is not a whole number of stages takes zeros behind it.
+template <class TL, class T, bool AKC, bool BKC>
+struct Stream {
+  using OA = Operand<T, AKC, TL::BN, kPer16<T>>;
+  using OB = Operand<T, BKC, TL::BM, 4>;
+  static constexpr int ES = (int)sizeof(T), KSTEP = OA::KSTEP, P = TL::PA + TL::PB;
+  unsigned offset[P];
+  const char *base_a, *base_b;
+  int left_k;              // behind the next stage's first k
+  unsigned lds_a, lds_b, slot;  // slot: the next stage's buffer, byte 0 or byte STAGE
 
-  const int wn = (wv % TL::WN) * TL::TN, wm = (wv / TL::WN) * TL::TM;
-  u4 fa[TL::RN], fb[TL::RM];
-  auto read = [&](const unsigned char* stage, int sub) {
-#pragma unroll
-    for (int j = 0; j < TL::RM; ++j) fb[j] = OB::fragment(stage + TL::A_BYTES, wm + 16 * j, sub, lane);
-#pragma unroll
-    for (int i = 0; i < TL::RN; ++i)
-      fa[i] = OA::fragment(stage, wn + 16 * HALF * (i / HALF) + 4 * (i % HALF), sub, lane);
-  };
-  auto multiply = [&] {
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int i = 0; i < TL::RN; ++i)
-#pragma unroll
-      for (int j = 0; j < TL::RM; ++j) acc[i][j] = Mma<T>::step(fa[i], fb[j], acc[i][j]);
-    __builtin_amdgcn_s_setprio(0);
-  };
-
-  if constexpr (DMA) {
-    constexpr int P = TL::PA + TL::PB;
-    // A piece's place is a uniform base that moves with k and a fixed offset per lane.  Rows outside the
-    // operand repeat the last one (their results are never stored); the last stage of a k that is not a
-    // whole number of stages takes zeros behind it.
-    unsigned offset[P];
-    int at_k[P];
+  __device__ __forceinline__ static void where(int i, int wv, int lane, int& row, int& k) {
+    if (i < TL::PA) OA::where((TL::PA * wv + i) * 64 + lane, row, k);
+    else OB::where((TL::PB * wv + i - TL::PA) * 64 + lane, row, k);
+  }
+  __device__ __forceinline__ void init(const unsigned char* smem, int wv) {
+    const unsigned lds0 = (unsigned)(unsigned long long)smem;
+    lds_a = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + (unsigned)(TL::PA * wv) * 1024u));
+    lds_b = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + TL::A_BYTES + (unsigned)(TL::PB * wv) * 1024u));
+    slot = 0;
+  }
+  // start and the rare part of issue work places out anew: without that the compiler would keep them in
+  // registers that the matrix loop needs.
+  static __device__ __forceinline__ int anew(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+  }
+  __device__ __forceinline__ void start(const Gemm& p, const Place& w, int wv, int lane) {
+    lane = anew(lane);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const bool isa = i < TL::PA, kc = isa ? AKC : BKC;
-      const int s = (isa ? TL::PA * wv + i : TL::PB * wv + i - TL::PA) * 64 + lane;
       int row, k;
-      if (isa) OA::where(s, row, k);
-      else OB::where(s, row, k);
-      row = min(row, (isa ? p.n - n0 : p.m - m0) - (kc ? 1 : OA::V));
+      where(i, wv, lane, row, k);
+      row = min(row, (isa ? p.n - w.n0 : p.m - w.m0) - (kc ? 1 : OA::V));
       const long long ld = isa ? p.lda : p.ldb;
       offset[i] = (unsigned)((kc ? row * ld + k : k * ld + row) * ES);
-      at_k[i] = k;
     }
-    const char* base_a = static_cast<const char*>(p.a) + (AKC ? n0 * p.lda + k_begin : k_begin * p.lda + n0) * ES;
-    const char* base_b = static_cast<const char*>(p.b) + (BKC ? m0 * p.ldb + k_begin : k_begin * p.ldb + m0) * ES;
-    const long long step_a = (AKC ? (long long)KSTEP : KSTEP * p.lda) * ES;
-    const long long step_b = (BKC ? (long long)KSTEP : KSTEP * p.ldb) * ES;
-    int left_k = k_end - k_begin;  // behind the next stage's first k
-    const unsigned lds0 = (unsigned)(unsigned long long)(smem);
-    const unsigned lds_a = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + (unsigned)(TL::PA * wv) * 1024u));
-    const unsigned lds_b = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds0 + TL::A_BYTES + (unsigned)(TL::PB * wv) * 1024u));
-    unsigned slot = 0;  // the two stages: byte 0 and byte STAGE
-    auto issue = [&] {
+    base_a = static_cast<const char*>(p.a) + (AKC ? w.n0 * p.lda + w.k_begin : w.k_begin * p.lda + w.n0) * ES;
+    base_b = static_cast<const char*>(p.b) + (BKC ? w.m0 * p.ldb + w.k_begin : w.k_begin * p.ldb + w.m0) * ES;
+    left_k = w.k_end - w.k_begin;
+  }
+  __device__ __forceinline__ void issue(const Gemm& p, int wv, int lane) {
+    const unsigned to_a = (unsigned)__builtin_amdgcn_readfirstlane((int)(slot + lds_a));
+    const unsigned to_b = (unsigned)__builtin_amdgcn_readfirstlane((int)(slot + lds_b));
+    if (left_k >= KSTEP) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const bool isa = i < TL::PA;
-        const char* base = isa ? base_a : base_b;
-        const unsigned dst = slot + (isa ? lds_a + 1024u * i : lds_b + 1024u * (i - TL::PA));
-        if (left_k >= KSTEP) dma16(base, offset[i], dst);
-        else dma16(at_k[i] < left_k ? base + offset[i] : reinterpret_cast<const char*>(kZeros), dst);
-      }
-      base_a += step_a, base_b += step_b;
-      left_k -= KSTEP;
-      slot ^= TL::STAGE;
-    };
-    if constexpr (TL::NW == 8) {
-      // Two waves share a SIMD.  The waves of the second half run one phase behind: while one wave of
-      // a SIMD reads its fragments, the other one multiplies, so that neither the LDS nor the matrix
-      // cores wait for the other.  Barriers keep the phases.  Of stage s, with both steps:
-      //   first half    read 0 | multiply 0 | read 1     | multiply 1 | read 0 of s + 1
-      //   second half          | read 0     | multiply 0 | read 1     | multiply 1
-      // Buffer s is free when the second half has done read 1; from there to the first half's next
-      // read of that buffer lie four phases, in which its next stage arrives.
-      const bool second = wv >= 4;
-      issue();
-      if (steps > 1) issue();
-      if (steps > 1) wait_loads<P>();
-      else wait_loads<0>();
-      barrier_keep_loads();
-      if (second) barrier_keep_loads();
-      for (int s = 0; s < steps; ++s) {
-        const unsigned char* stage = smem + (s & 1) * TL::STAGE;
-        if (!second && s > 0 && s + 1 < steps) issue();
-        read(stage, 0);
-        wait_loads<63>();
-        barrier_keep_loads();
-        multiply();
-        barrier_keep_loads();
-        read(stage, 1);
-        if (second) wait_loads<0>();
-        else wait_loads<63>();
-        barrier_keep_loads();
-        if (second && s + 2 < steps) issue();
-        multiply();
-        if (!second) wait_loads<0>();
-        barrier_keep_loads();
-      }
-      if (!second) barrier_keep_loads();
+      for (int i = 0; i < P; ++i)
+        dma16(i < TL::PA ? base_a : base_b, offset[i], i < TL::PA ? to_a + 1024u * i : to_b + 1024u * (i - TL::PA));
     } else {
-      issue();
-      for (int s = 0; s < steps; ++s) {
-        // stage s has landed for this wave; the barrier makes that all waves, and no wave still reads
-        // the buffer that the next loads go to
-        const unsigned char* stage = smem + (s & 1) * TL::STAGE;
-        wait_loads<0>();
-        barrier_keep_loads();
-        if (s + 1 < steps) issue();
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          read(stage, sub);
-          multiply();
-        }
-      }
-    }
-    wait_loads<0>();
-  } else {
-    constexpr int P = TL::PA + TL::PB;
-    u4 held[P];
-    auto fetch = [&](int step) {
+      lane = anew(lane);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const bool isa = i < TL::PA;
-        const int s = (isa ? TL::PA * wv + i : TL::PB * wv + i - TL::PA) * 64 + lane;
         int row, k;
-        if (isa) OA::where(s, row, k);
-        else OB::where(s, row, k);
-        row += isa ? n0 : m0;
-        k += k_begin + step * KSTEP;
-        const int rows = isa ? p.n : p.m;
-        const long long ld = isa ? p.lda : p.ldb;
-        const T* base = static_cast<const T*>(isa ? p.a : p.b);
-        const bool kc = isa ? AKC : BKC;
-        held[i] = u4{0, 0, 0, 0};
-        if (kc) {
-          if (row < rows && k < k_end) held[i] = load_piece(base + row * ld + k, k_end - k);
-        } else {
-          if (row < rows && k < k_end) held[i] = load_piece(base + k * ld + row, rows - row);
-        }
-      }
-    };
-    fetch(0);
-    for (int s = 0; s < steps; ++s) {
-      unsigned char* stage = smem + (s & 1) * TL::STAGE;
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const bool isa = i < TL::PA;
-        const int at = (isa ? TL::PA * wv + i : TL::PB * wv + i - TL::PA) * 1024 + lane * 16 + (isa ? 0 : TL::A_BYTES);
-        *reinterpret_cast<u4*>(stage + at) = held[i];
-      }
-      __syncthreads();  // this stage is written; every wave is done with the other one
-      if (s + 1 < steps) fetch(s + 1);
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        read(stage, sub);
-        multiply();
+        where(i, wv, lane, row, k);
+        const char* base = i < TL::PA ? base_a : base_b;
+        dma16(k < left_k ? base + offset[i] : reinterpret_cast<const char*>(kZeros),
+              i < TL::PA ? to_a + 1024u * i : to_b + 1024u * (i - TL::PA));
       }
     }
+    base_a += (AKC ? (long long)KSTEP : KSTEP * p.lda) * ES;
+    base_b += (BKC ? (long long)KSTEP : KSTEP * p.ldb) * ES;
+    left_k -= KSTEP;
+    slot ^= TL::STAGE;
+  }
+};
+
+// A wave's part of the tile: its accumulators, and the two halves of a matrix step.
+template <class TL, class T, bool AKC, bool BKC>
+struct Part {
+  static constexpr int HALF = kPer16<T> / 4;  // accumulators that make up 16 bytes of a lane
+  using OA = Operand<T, AKC, TL::BN, 4 * HALF>;
+  using OB = Operand<T, BKC, TL::BM, 4>;
+  f4 acc[TL::RN][TL::RM];
+  // fragments of one matrix step: the second operand's (two steps' worth: the next step's arrive while
+  // this one's are used) and one half of the first operand's at a time, likewise twice
+  static constexpr int RH = TL::RN / 2;
+  u4 fa[2][RH], fb[2][TL::RM];
+  int wn, wm, lane;
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < TL::RN; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::RM; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  __device__ __forceinline__ void init(int wv, int lane_) {
+    wn = (wv % TL::WN) * TL::TN, wm = (wv / TL::WN) * TL::TM, lane = lane_;
+    clear();
+  }
+  __device__ __forceinline__ void read_b(const unsigned char* stage, int sub) {
+#pragma unroll
+    for (int j = 0; j < TL::RM; ++j) fb[sub & 1][j] = OB::fragment(stage + TL::A_BYTES, wm + 16 * j, sub, lane);
+  }
+  __device__ __forceinline__ void read_a(const unsigned char* stage, int sub, int half) {
+#pragma unroll
+    for (int h = 0; h < RH; ++h) {
+      const int i = half * RH + h;
+      fa[half][h] = OA::fragment(stage, wn + 16 * HALF * (i / HALF) + 4 * (i % HALF), sub, lane);
+    }
+  }
+  __device__ __forceinline__ void multiply(int sub, int half) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int h = 0; h < RH; ++h)
+#pragma unroll
+      for (int j = 0; j < TL::RM; ++j)
+        acc[half * RH + h][j] = Mma<T>::step(fa[half][h], fb[sub & 1][j], acc[half * RH + h][j]);
+    __builtin_amdgcn_s_setprio(0);
+  }
+  // One stage, beginning with read_b(stage, 0) and read_a(stage, 0, 0) done: every read goes out half
+  // a step (RH x RM matrix instructions) before its use.  `turn` is called once all reads of the stage
+  // have arrived; it may start the next stage's.
+  template <class F>
+  __device__ __forceinline__ void run_stage(const unsigned char* stage, F turn) {
+    read_a(stage, 0, 1);
+    multiply(0, 0);
+    read_b(stage, 1);
+    read_a(stage, 1, 0);
+    multiply(0, 1);
+    read_a(stage, 1, 1);
+    multiply(1, 0);
+    turn();
+    multiply(1, 1);
+  }
+  __device__ __forceinline__ void begin_stage(const unsigned char* stage) {
+    read_b(stage, 0);
+    read_a(stage, 0, 0);
   }
 
   // accumulators HALF i ...: columns n0 + wn + 16 HALF i + V g ... of row m0 + wm + 16 j + (lane & 15)
-  constexpr int V = kPer16<T>, NP = TL::RN / HALF;
-  const int g = lane >> 4;
-  const int n_first = n0 + wn + V * g;
-  auto finish_tile = [&](auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;  // no edge of the result inside this tile
-    float bias[NP][V];
-    u4 res[NP];
+  static constexpr int V = kPer16<T>, NP = TL::RN / HALF;
+  // the vector stores of a tile without edges are at least this many
+  static constexpr int STORES = TL::RM * NP;
+  template <bool WHOLE, int ACT, bool PLUS>  // WHOLE: no edge of the result inside this tile
+  __device__ __forceinline__ void finish_tile(const Gemm& p, const Place& w) {
+    const int n_first = w.n0 + wn + V * (lane >> 4);
+    const int m_first = w.m0 + wm + (lane & 15);
     auto left_of = [&](int i) { return WHOLE ? V : p.n - (n_first + 16 * HALF * i); };
-    // loads of a row's pieces go out together, and ahead of the stores of the row before
-    auto fetch = [&](int j) {
-      const long long m = m0 + wm + 16 * j + (lane & 15);
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        res[i] = load_residual<T>(p.e, m, n_first + 16 * HALF * i, WHOLE || m < p.m ? left_of(i) : 0);
+    auto residual = [&](int i, int j) {
+      if constexpr (PLUS) {
+        const int m = m_first + 16 * j;
+        return load_residual<T>(p.e, m, n_first + 16 * HALF * i, WHOLE || m < p.m ? left_of(i) : 0);
+      }
+      return u4{0, 0, 0, 0};
     };
+    T* const out = static_cast<T*>(p.e.out) + (long long)m_first * p.n + n_first;
+    T* const z = p.e.z ? static_cast<T*>(p.e.z) + (long long)m_first * p.n + n_first : nullptr;
+    const long long step = 16LL * p.n;
+    // bias and residual are loaded one piece ahead of the stores
+    float next_bias[V];
+    u4 next = residual(0, 0);
+    load_bias<T>(p.e, n_first, left_of(0), next_bias);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) load_bias<T>(p.e, n_first + 16 * HALF * i, left_of(i), bias[i]);
-    if (p.e.residual) fetch(0);
+    for (int i = 0; i < NP; ++i) {
+      float bias[V];
 #pragma unroll
-    for (int j = 0; j < TL::RM; ++j) {
-      const long long m = m0 + wm + 16 * j + (lane & 15);
-      u4 now[NP];
+      for (int t = 0; t < V; ++t) bias[t] = next_bias[t];
+      if (i + 1 < NP) load_bias<T>(p.e, n_first + 16 * HALF * (i + 1), left_of(i + 1), next_bias);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) now[i] = res[i];
-      if (p.e.residual && j + 1 < TL::RM) fetch(j + 1);
-      if (!WHOLE && m >= p.m) continue;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (!WHOLE && left_of(i) <= 0) continue;
+      for (int j = 0; j < TL::RM; ++j) {
+        const u4 now = next;
+        if (j + 1 < TL::RM) next = residual(i, j + 1);
+        else if (i + 1 < NP) next = residual(i + 1, 0);
+        if (!WHOLE && (m_first + 16 * j >= p.m || left_of(i) <= 0)) continue;
         float v[V];
 #pragma unroll
         for (int t = 0; t < V; ++t) v[t] = acc[HALF * i + t / 4][j][t % 4];
-        finish<T>(p.e, m * p.n + n_first + 16 * HALF * i, left_of(i), bias[i], now[i], v);
+        const long long at = j * step + 16 * HALF * i;
+        finish<T, ACT, PLUS>(out + at, z ? z + at : nullptr, left_of(i), bias, now, v);
       }
     }
-  };
-  if (p.splits > 1) {
+  }
+  __device__ __forceinline__ void store_part(const Gemm& p, const Place& w) {
+    const int n_first = w.n0 + wn + V * (lane >> 4);
 #pragma unroll
     for (int j = 0; j < TL::RM; ++j) {
-      const long long m = m0 + wm + 16 * j + (lane & 15);
+      const long long m = w.m0 + wm + 16 * j + (lane & 15);
       if (m >= p.m) continue;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -466,15 +452,171 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
         float v[V];
 #pragma unroll
         for (int t = 0; t < V; ++t) v[t] = acc[HALF * i + t / 4][j][t % 4];
-        float* out = p.partial + ((long long)split * p.m + m) * p.n + n;
+        float* out = p.partial + ((long long)w.split * p.m + m) * p.n + n;
 #pragma unroll
         for (int t = 0; t < V; t += 4) store_piece(out + t, pack<float>(v + t), left - t);
       }
     }
-  } else if (n0 + TL::BN <= p.n && m0 + TL::BM <= p.m) {
-    finish_tile(std::true_type());
+  }
+  static __device__ __forceinline__ bool whole(const Gemm& p, const Place& w) {
+    return w.n0 + TL::BN <= p.n && w.m0 + TL::BM <= p.m;
+  }
+  __device__ __forceinline__ void store(const Gemm& p, const Place& w) {
+    if (p.splits > 1) {
+      store_part(p, w);
+    } else if constexpr (!AKC) {  // a gradient
+      if (whole(p, w)) finish_tile<true, MIA_ACT_NONE, false>(p, w);
+      else finish_tile<false, MIA_ACT_NONE, false>(p, w);
+    } else if (whole(p, w)) {
+      with_epilogue(p.e, [&](auto act, auto plus) { finish_tile<true, decltype(act)::value, decltype(plus)::value>(p, w); });
+    } else {
+      with_epilogue(p.e, [&](auto act, auto plus) { finish_tile<false, decltype(act)::value, decltype(plus)::value>(p, w); });
+    }
+    if (!whole(p, w)) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): pieces outside were loaded and not used
+  }
+};
+}  // namespace lin
+
+// Four waves, one tile per workgroup; several workgroups share a compute unit and fill each other's
+// gaps.  DMA: every 16-byte piece of both operands is aligned (bases, row strides) and lies either
+// wholly inside its operand or wholly outside; otherwise pieces go through registers, element by
+// element at the edges.
+template <class TL, class T, bool AKC, bool BKC, bool DMA>
+__global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) {
+  using namespace lin;
+  using ST = Stream<TL, T, AKC, BKC>;
+  constexpr int KSTEP = ST::KSTEP, P = ST::P;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned first, count;
+  xcd_share(gridDim.x, blockIdx.x & 7, first, count);
+  const Place w = place<TL>(p, first + (blockIdx.x >> 3));
+  const int steps = (w.k_end - w.k_begin + KSTEP - 1) / KSTEP;
+  Part<TL, T, AKC, BKC> part;
+  part.init(wv, lane);
+
+  if constexpr (DMA) {
+    ST st;
+    st.init(smem, wv);
+    st.start(p, w, wv, lane);
+    if (steps > 0) st.issue(p, wv, lane);
+    if (steps > 1) st.issue(p, wv, lane);
+    if (steps > 1) wait_loads<P>();
+    else wait_loads<0>();
+    barrier_keep_loads();
+    if (steps > 0) part.begin_stage(smem);
+    for (int s = 0; s < steps; ++s) {
+      part.run_stage(smem + (s & 1) * TL::STAGE, [&] {
+        if (s + 1 == steps) return;
+        // stage s + 1 has landed for this wave, and its reads of stage s have arrived; the barrier makes
+        // that all waves: stage s + 2 may go where stage s was
+        wait_loads<0>();
+        barrier_keep_loads();
+        if (s + 2 < steps) st.issue(p, wv, lane);
+        part.begin_stage(smem + ((s + 1) & 1) * TL::STAGE);
+      });
+    }
   } else {
-    finish_tile(std::false_type());
+    u4 held[P];
+    auto fetch = [&](int step) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const bool isa = i < TL::PA, kc = isa ? AKC : BKC;
+        int row, k;
+        ST::where(i, wv, lane, row, k);
+        row += isa ? w.n0 : w.m0;
+        k += w.k_begin + step * KSTEP;
+        const int rows = isa ? p.n : p.m;
+        const long long ld = isa ? p.lda : p.ldb;
+        const T* base = static_cast<const T*>(isa ? p.a : p.b);
+        held[i] = u4{0, 0, 0, 0};
+        if (row < rows && k < w.k_end)
+          held[i] = kc ? load_piece(base + row * ld + k, w.k_end - k) : load_piece(base + k * ld + row, rows - row);
+      }
+    };
+    if (steps > 0) fetch(0);
+    for (int s = 0; s < steps; ++s) {
+      unsigned char* stage = smem + (s & 1) * TL::STAGE;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int at = i < TL::PA ? (TL::PA * wv + i) * 1024 : TL::A_BYTES + (TL::PB * wv + i - TL::PA) * 1024;
+        *reinterpret_cast<u4*>(stage + at + lane * 16) = held[i];
+      }
+      __syncthreads();  // this stage is written; every wave is done with the other one
+      if (s + 1 < steps) fetch(s + 1);
+      part.begin_stage(stage);
+      part.run_stage(stage, [] {});
+    }
+  }
+  part.store(p, w);
+}
+
+// Eight waves, one workgroup per compute unit, which walks tiles (of one XCD's share) without a break
+// in its stream of loads: stage g + 2 of the stream, which may be the next tile's, is loaded into the
+// buffer of stage g as soon as all waves have read that, one stage before its use.  So at the end of
+// a tile the results are stored while the next tile's first stages arrive; a wave waits for its loads,
+// never for the stores behind them (loads and stores are counted in order: "all but the newest STORES").
+template <class TL, class T, bool AKC, bool BKC>
+__global__ __launch_bounds__(TL::WG, 1) void lin_gemm8_kernel(lin::Gemm p) {
+  using namespace lin;
+  using ST = Stream<TL, T, AKC, BKC>;
+  using PT = Part<TL, T, AKC, BKC>;
+  constexpr int KSTEP = ST::KSTEP;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned first, count;
+  xcd_share((unsigned)p.n_tiles * p.m_tiles * p.splits, blockIdx.x & 7, first, count);
+  const unsigned stride = (gridDim.x + 7 - (blockIdx.x & 7)) / 8;  // workgroups on this XCD
+  unsigned at = blockIdx.x >> 3;                                   // index in the XCD's share
+  if (at >= count) return;
+
+  Place w = place<TL>(p, first + at);
+  PT part;
+  part.init(wv, lane);
+  ST st;
+  st.init(smem, wv);
+  // the stream's own position: it is up to two stages, possibly a tile, ahead
+  unsigned load_at = at;
+  st.start(p, w, wv, lane);
+  bool more = true;
+  auto issue = [&] {
+    if (!more) return;
+    st.issue(p, wv, lane);
+    if (st.left_k <= 0) {
+      load_at += stride;
+      more = load_at < count;
+      if (more) st.start(p, place<TL>(p, first + load_at), wv, lane);
+    }
+  };
+  issue();
+  issue();
+  wait_loads<0>();
+  barrier_keep_loads();
+  unsigned buffer = 0;
+  bool stored = false;  // stores of a whole tile are behind this wave's newest loads
+  for (;;) {
+    const int steps = (w.k_end - w.k_begin + KSTEP - 1) / KSTEP;
+    part.begin_stage(smem + buffer);
+    for (int s = 0; s < steps; ++s) {
+      part.run_stage(smem + buffer, [&] {
+        // this wave's reads of the stage and its loads of the next one have arrived; then all waves'
+        if (stored) wait_loads<PT::STORES>();
+        else wait_loads<0>();
+        stored = false;
+        barrier_keep_loads();
+        issue();
+        buffer ^= TL::STAGE;
+        if (s + 1 < steps) part.begin_stage(smem + buffer);
+      });
+    }
+    part.store(p, w);
+    stored = PT::whole(p, w);
+    at += stride;
+    if (at >= count) break;
+    w = place<TL>(p, first + at);
+    part.clear();
   }
 }
 
@@ -491,7 +633,7 @@ __global__ __launch_bounds__(256) void lin_join_kernel(lin::Gemm p) {
     const int left = p.n - n;
     float b[V], v[V] = {};
     load_bias<T>(p.e, n, left, b);
-    const u4 r = load_residual<T>(p.e, m, n, left);
+    const u4 r = p.e.residual ? load_residual<T>(p.e, m, n, left) : u4{0, 0, 0, 0};
     for (int s = 0; s < p.splits; ++s) {
       const float* src = p.partial + ((long long)s * p.m + m) * p.n + n;
 #pragma unroll
@@ -502,7 +644,11 @@ __global__ __launch_bounds__(256) void lin_join_kernel(lin::Gemm p) {
         for (int j = 0; j < 4; ++j) v[t + j] += x[j];
       }
     }
-    finish<T>(p.e, m * p.n + n, left, b, r, v);
+    T* out = static_cast<T*>(p.e.out) + m * p.n + n;
+    T* z = p.e.z ? static_cast<T*>(p.e.z) + m * p.n + n : nullptr;
+    with_epilogue(p.e, [&](auto act, auto plus) {
+      finish<T, decltype(act)::value, decltype(plus)::value>(out, z, left, b, r, v);
+    });
   }
 }
 
@@ -657,13 +803,15 @@ static int launch(Gemm g, hipStream_t s) {
     set_error("product too large for one launch");
     return MIA_ERR_UNSUPPORTED;
   }
-  constexpr int lds = TL::LDS;
-  auto kern = lin_gemm_kernel<TL, T, AKC, BKC, DMA>;
-  if constexpr (lds > 64 * 1024) {
-    MIA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  }
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(TL::WG), lds, s, g);
-  return MIA_OK;
+  auto run = [&](auto kern, unsigned grid) {
+    if constexpr (TL::LDS > 64 * 1024) {
+      MIA_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, TL::LDS));
+    }
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(TL::WG), TL::LDS, s, g);
+    return MIA_OK;
+  };
+  if constexpr (TL::NW == 8) return run(lin_gemm8_kernel<TL, T, AKC, BKC>, (unsigned)(blocks < kCus ? blocks : kCus));
+  else return run(lin_gemm_kernel<TL, T, AKC, BKC, DMA>, (unsigned)blocks);
 }
 
 template <class T, bool AKC, bool BKC>

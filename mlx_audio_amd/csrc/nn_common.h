@@ -129,6 +129,8 @@ __device__ __forceinline__ void dma16(const void* gptr, unsigned lds_byte_addr) 
       : "memory");
 }
 // the same from a uniform base and a lane's unsigned byte offset: no address arithmetic per lane
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the compiler keeps nothing in it
 __device__ __forceinline__ void dma16(const void* base, unsigned offset, unsigned lds_byte_addr) {
   asm volatile(
       "s_mov_b32 m0, %2\n\t"
@@ -138,6 +140,7 @@ __device__ __forceinline__ void dma16(const void* base, unsigned offset, unsigne
       : "s"(base), "v"(offset), "s"(lds_byte_addr)
       : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // the same with 4 bytes a lane, at lds_byte_addr + 4 L
 __device__ __forceinline__ void dma4(const void* gptr, unsigned lds_byte_addr) {
   unsigned keep;
