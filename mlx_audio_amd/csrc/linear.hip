@@ -48,7 +48,7 @@ extern "C" {
 
 size_t mia_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
   if (rows <= lin::kFewRows || in <= 0 || out <= 0 || !nn::dtype_ok(dtype)) return 0;
-  return lin::split_bytes(out, rows, in, nn::dtype_size(dtype));
+  return lin::split_bytes(out, rows, in, nn::dtype_size(dtype), false);
 }
 
 int mia_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
@@ -80,7 +80,7 @@ size_t mia_linear_backward_workspace_bytes(int64_t rows, int64_t in, int64_t out
   const size_t es = nn::dtype_size(dtype);
   const size_t dz = activation == MIA_ACT_NONE ? 0 : nn::align256((size_t)rows * out * es);
   const size_t bias = nn::align256((size_t)lin::bias_groups(rows) * out * sizeof(float));
-  const size_t dx = lin::split_bytes(in, rows, out, es), dw = lin::split_bytes(in, out, rows, es);
+  const size_t dx = lin::split_bytes(in, rows, out, es, false), dw = lin::split_bytes(in, out, rows, es, true);
   return dz + bias + (dx > dw ? dx : dw);
 }
 

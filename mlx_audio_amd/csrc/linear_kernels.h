@@ -774,24 +774,49 @@ static long long tiles_of(long long n, long long m, int tile) {
   return ((n + tile - 1) / tile) * ((m + tile - 1) / tile);
 }
 
-// The tile and the number of parts of k, from the sizes alone (the workspace size follows from it).
-static Choice choose(long long n, long long m, long long k, size_t es, bool dma) {
+// The tile and the number of parts of k: the pair with the least estimated time, from the sizes alone
+// (the workspace size follows from it).  The estimate is rounds of workgroups x (stages x time of a
+// stage + start and end), and the join of the parts; its constants, in us, were measured with every
+// tile forced in turn (bfloat16 / float32, all compute units busy):
+//   256 x 256, one workgroup per compute unit:  1.6 / 7.2 a stage (1.8 / 11 with both operands by columns)
+//   128 x 128, two:                             0.88 / 3.6
+//   64 x 64, four:                              0.83 / 1.8
+// e.g. 24000 x 1280 -> 1280: 256 75 us, 128 87, 64 121;  6000 x 1280 -> 1280: 36, 25, 36;
+// 1500 x 1280 -> 1280: 128 18.5, 64 14.0;  1500 x 5120 -> 1280: 128 in 4 parts 34.8, in 2 38.0.
+static Choice choose(long long n, long long m, long long k, size_t es, bool dma, bool columns) {
+  struct Kind {
+    int tile, per_cu;
+    double stage2, stage4, ends;
+  };
+  static const Kind kinds[3] = {{256, 1, 1.6, 7.2, 6.0}, {128, 2, 0.88, 3.6, 4.0}, {64, 4, 0.83, 1.8, 3.0}};
   const int kstep = (int)(128 / es);
   const long long steps = (k + kstep - 1) / kstep;
-  Choice c{64, 1, 0};
-  if (dma && tiles_of(n, m, 256) >= kCus) c.tile = 256;
-  else if (tiles_of(n, m, 128) >= kCus / 2) c.tile = 128;
-  const long long tiles = tiles_of(n, m, c.tile);
-  const long long fill = c.tile == 256 ? kCus : c.tile == 128 ? 2 * kCus : 4 * kCus;
-  long long splits = 1;
-  if (tiles < fill) splits = fill / tiles;
-  if (splits > steps / 8) splits = steps / 8;
-  if (splits > 32) splits = 32;
-  if (splits < 1) splits = 1;
-  const long long per = steps ? (steps + splits - 1) / splits : 1;
-  c.splits = steps ? (int)((steps + per - 1) / per) : 1;
-  c.k_per_split = (int)(per * kstep);
-  return c;
+  Choice best{64, 1, 0};
+  double least = 0.0;
+  for (const Kind& kd : kinds) {
+    if (kd.tile == 256 && !dma) continue;
+    const long long tiles = tiles_of(n, m, kd.tile);
+    for (int splits = 1; splits <= 32 && (splits == 1 || steps / splits >= 4); ++splits) {
+      const long long groups = tiles * splits, per_cu = (groups + kCus - 1) / kCus;
+      const double load = per_cu < kd.per_cu ? (double)per_cu / kd.per_cu : 1.0;  // a stage is faster alone
+      double stage = (es == 4 ? kd.stage4 : kd.stage2) * (0.45 + 0.55 * load);
+      if (kd.tile == 256) stage = es == 4 ? (columns ? 11.0 : kd.stage4) : (columns ? 1.8 : kd.stage2);
+      const long long rounds = (groups + (long long)kCus * kd.per_cu - 1) / ((long long)kCus * kd.per_cu);
+      double t = (double)rounds * ((double)((steps + splits - 1) / splits) * stage + kd.ends);
+      if (splits > 1) {  // parts written and read: 8 TB/s while the caches hold them, half of that beyond
+        const double mb = 8e-6 * (double)splits * (double)m * (double)n;
+        t += 6.0 + mb / 8.0 + (mb > 64.0 ? (mb - 64.0) / 8.0 : 0.0);
+      }
+      if (least == 0.0 || t < least) {
+        least = t;
+        best.tile = kd.tile, best.splits = splits;
+      }
+    }
+  }
+  const long long per = steps ? (steps + best.splits - 1) / best.splits : 1;
+  best.splits = steps ? (int)((steps + per - 1) / per) : 1;
+  best.k_per_split = (int)(per * kstep);
+  return best;
 }
 
 template <class TL, class T, bool AKC, bool BKC, bool DMA>
@@ -816,7 +841,7 @@ static int launch(Gemm g, hipStream_t s) {
 
 template <class T, bool AKC, bool BKC>
 static int gemm(const Operands& o, const Epilogue& e, void* workspace, bool dma, hipStream_t s) {
-  const Choice c = choose(o.n, o.m, o.k, sizeof(T), dma);
+  const Choice c = choose(o.n, o.m, o.k, sizeof(T), dma, !AKC && !BKC);
   Gemm g{o.a, o.b, o.lda, o.ldb, (int)o.n, (int)o.m, (int)o.k, 0, 0, c.splits, c.k_per_split,
          static_cast<float*>(workspace), e};
   int rc;
@@ -842,11 +867,11 @@ static bool pieces_ok(const void* p, long long ld, long long contiguous, size_t 
   return aligned16(p) && ld % v == 0 && contiguous % v == 0 && ld * (long long)es < (1LL << 24);
 }
 
-static size_t split_bytes(long long n, long long m, long long k, size_t es) {
+static size_t split_bytes(long long n, long long m, long long k, size_t es, bool columns) {
   // both ways of loading may be taken (alignment is not known here): the larger of the two
   size_t most = 0;
   for (int dma = 0; dma < 2; ++dma) {
-    const Choice c = choose(n, m, k, es, dma != 0);
+    const Choice c = choose(n, m, k, es, dma != 0, columns);
     const size_t need = c.splits > 1 ? (size_t)c.splits * m * n * sizeof(float) : 0;
     most = need > most ? need : most;
   }
