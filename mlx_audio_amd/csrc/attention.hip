@@ -91,9 +91,9 @@ int mia_attention_backward(const mia_attention_desc* d, const void* dout, const 
   MIA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && nn::aligned16(workspace)), "workspace too small");
   att::Args a = att::args(d, q, k, v, key_lengths);
   a.dout = att::view(dout, stride_dout), a.out = att::view(out, stride_out);
+  a.lse = const_cast<float*>(lse);
   const int done = nn::with_dtype(d->dtype, [&](auto t) {
-    return att::Ops<decltype(t)>::backward(a, lse, static_cast<float*>(workspace), dq, dk, dv,
-                                           static_cast<hipStream_t>(stream));
+    return att::Ops<decltype(t)>::backward(a, static_cast<float*>(workspace), dq, dk, dv, static_cast<hipStream_t>(stream));
   });
   if (done != MIA_OK) return done;
   MIA_CHECK_HIP(hipGetLastError());

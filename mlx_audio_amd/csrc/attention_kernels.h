@@ -31,8 +31,9 @@ struct Args {
   View q, k, v, out, dout;
   void* o0;           // forward: out; dq; dk          (contiguous [batch, row, head, dim])
   void* o1;           // dv
-  float* lse;         // (batch, heads, sq): written by the forward
-  const float* stats; // backward: lse / ln 2 (+inf for an empty row), then delta, (batch, heads, sq) each
+  float* lse;         // (batch, heads, sq): written by the forward, read by the backward
+  float* stats;       // backward: lse / ln 2 (+inf for an empty row), then delta, (batch, heads, sq) each;
+                      // dq writes them, dk / dv reads them
   const int* lengths; // (batch) keys of each batch item, or null
   int batch, sq, sk, heads, kv_heads, dim;
   int pack;           // heads that share a workgroup's rows: 1, or heads / kv_heads (few queries)
@@ -462,41 +463,8 @@ __global__ __launch_bounds__(256) void att_join_kernel(att::Args p) {
   if (lane == 0 && p.lse) p.lse[at] = total == 0.0f ? -kInf : fmaf(top, kLn2, logf(total));
 }
 
+// dq: own rows are queries, k and v stream.  Runs first and leaves for dk / dv what each query needs there:
 // stats[0] = lse / ln 2 (+inf for an empty row: its p becomes 0), stats[1] = delta = sum_d dout out.
-// 16 lanes per row, rows in memory order.
-template <class T>
-__global__ __launch_bounds__(256) void att_stats_kernel(att::Args p, const float* __restrict__ lse,
-                                                        float* __restrict__ stats) {
-  using namespace att;
-  constexpr int V = kPer16<T>;
-  const long long n = (long long)p.batch * p.heads * p.sq;
-  const long long r = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int l = threadIdx.x & 15;
-  if (r >= n) return;
-  const int h = (int)(r % p.heads);
-  const long long bs = r / p.heads, b = bs / p.sq;
-  const int s = (int)(bs - b * p.sq);
-  const T* o = static_cast<const T*>(p.out.p) + b * p.out.b + s * p.out.s + h * p.out.h;
-  const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.b + s * p.dout.s + h * p.dout.h;
-  float d = 0.0f;
-  for (int e = l * V; e < p.dim; e += 16 * V) {
-    float x[V], y[V];
-    unpack<T>(load_piece(o + e, p.dim - e), x);
-    unpack<T>(load_piece(g + e, p.dim - e), y);
-#pragma unroll
-    for (int j = 0; j < V; ++j) d = fmaf(x[j], y[j], d);
-  }
-#pragma unroll
-  for (int k = 8; k; k >>= 1) d += __shfl_xor(d, k);
-  if (l == 0) {
-    const long long at = (b * p.heads + h) * p.sq + s;
-    const float v = lse[at];
-    stats[at] = v == -kInf ? kInf : v * kLog2e;
-    stats[n + at] = d;
-  }
-}
-
-// dq: own rows are queries, k and v stream.
 template <class T, int DP, int OT, bool DMA>
 __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   using namespace att;
@@ -529,9 +497,25 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
     const bool in = s < p.sq;
     load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + h * p.q.h, in, p.dim, lane, oq[o]);
     load_own<T, DP>(static_cast<const T*>(p.dout.p) + b * p.dout.b + s * p.dout.s + h * p.dout.h, in, p.dim, lane, og[o]);
+    u4 oo[S::CC];
+    load_own<T, DP>(static_cast<const T*>(p.out.p) + b * p.out.b + s * p.out.s + h * p.out.h, in, p.dim, lane, oo);
+    float d = 0.0f;
+#pragma unroll
+    for (int cc = 0; cc < S::CC; ++cc) {
+      float x[S::V], y[S::V];
+      unpack<T>(oo[cc], x);
+      unpack<T>(og[o][cc], y);
+#pragma unroll
+      for (int j = 0; j < S::V; ++j) d = fmaf(x[j], y[j], d);
+    }
     const long long at = ((long long)b * p.heads + h) * p.sq + s;
-    lse2[o] = in ? p.stats[at] : kInf;
-    delta[o] = in ? p.stats[n + at] : 0.0f;
+    const float l = in ? p.lse[at] : -kInf;
+    delta[o] = column_sum(d);
+    lse2[o] = l == -kInf ? kInf : l * kLog2e;
+    if (in && g == 0 && split == 0) {
+      p.stats[at] = lse2[o];
+      p.stats[n + at] = delta[o];
+    }
     limit[o] = p.causal ? min(len, s + off + 1) : len;
   }
   f4 acc[S::DT][OT];
@@ -853,7 +837,7 @@ static size_t gradient_bytes(long long batch, long long sq, long long sk, int he
 template <class T>
 struct Ops {
   static int forward(Args a, hipStream_t s);
-  static int backward(Args a, const float* lse, float* stats, void* dq, void* dk, void* dv, hipStream_t s);
+  static int backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStream_t s);
 };
 #ifdef MIA_ATTENTION_TYPE
 // 16-byte pieces are aligned, a tile's rows lie within 32 bits of offset
@@ -894,17 +878,27 @@ int Ops<T>::forward(Args a, hipStream_t s) {
   return MIA_OK;
 }
 template <class T>
-int Ops<T>::backward(Args a, const float* lse, float* stats, void* dq, void* dk, void* dv, hipStream_t s) {
+int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStream_t s) {
   const long long rows = (long long)a.batch * a.heads * a.sq;
   const bool whole = a.dim % (16 / (int)sizeof(T)) == 0;
   a.stats = stats, a.pack = 1;
   a.partial = stats + align256((size_t)2 * rows * sizeof(float)) / sizeof(float);
-  if (rows) hipLaunchKernelGGL(att_stats_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, lse, stats);
   auto add = [&](const float* partial, long long stride, long long n, void* out) {
     const long long blocks = (n + 255) / 256;
     hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, partial,
                        stride, a.splits, n, static_cast<T*>(out));
   };
+  if (rows) {
+    const GradPlan pl = plan_dq(a.batch, a.sq, a.sk, a.heads, sizeof(T));
+    a.own_tiles = pl.own_tiles, a.splits = pl.splits;
+    a.o0 = dq, a.o1 = nullptr;
+    const unsigned grid = order_grid((long long)a.batch * a.heads, (long long)a.own_tiles * a.splits);
+    with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)), [&](auto dma) {
+      if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_dq_kernel, 2, grid);
+      else MIA_ATT_LAUNCH(att_dq_kernel, 1, grid);
+    });
+    if (a.splits > 1) add(a.partial, rows * a.dim, rows * a.dim, dq);
+  }
   if (a.sk) {
     const GradPlan pl = plan_dkv(a.batch, a.sq, a.sk, a.heads, a.kv_heads, a.dim, sizeof(T));
     a.own_tiles = pl.own_tiles, a.splits = pl.splits;
@@ -927,17 +921,6 @@ int Ops<T>::backward(Args a, const float* lse, float* stats, void* dq, void* dk,
       add(a.partial, 2 * n, n, dk);
       add(a.partial + n, 2 * n, n, dv);
     }
-  }
-  if (rows) {
-    const GradPlan pl = plan_dq(a.batch, a.sq, a.sk, a.heads, sizeof(T));
-    a.own_tiles = pl.own_tiles, a.splits = pl.splits;
-    a.o0 = dq, a.o1 = nullptr;
-    const unsigned grid = order_grid((long long)a.batch * a.heads, (long long)a.own_tiles * a.splits);
-    with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)), [&](auto dma) {
-      if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_dq_kernel, 2, grid);
-      else MIA_ATT_LAUNCH(att_dq_kernel, 1, grid);
-    });
-    if (a.splits > 1) add(a.partial, rows * a.dim, rows * a.dim, dq);
   }
   return MIA_OK;
 }

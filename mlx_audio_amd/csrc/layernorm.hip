@@ -254,26 +254,31 @@ __global__ __launch_bounds__(256) void ln_columns_kernel(ln::Args p) {
   p.partial[((long long)blockIdx.y * 2 + 1) * p.dim + i] = db;
 }
 
-// out[i] = sum over groups of partial[group][i], i < n, in order of the groups: 64 columns per
-// workgroup, each of its 16 waves a sixteenth of the groups.
+// out[i] = sum over groups of partial[group][i], i < n, in a fixed order: 32 columns per workgroup, each
+// of its 32 slices every 32nd group.
 __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__ partial, int groups, int n,
                                                        float* __restrict__ dw, float* __restrict__ db, int dim) {
-  __shared__ double part[16][64];
-  const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int i = blockIdx.x * 64 + lane;
-  double s = 0.0;
+  __shared__ double part[32][32];
+  const int slice = threadIdx.x >> 5, c = threadIdx.x & 31;
+  const int i = blockIdx.x * 32 + c;
+  double s[2] = {};
   if (i < n) {
-    const int per = (groups + 15) / 16;
-    const int end = min(groups, (wv + 1) * per);
-    for (int g = wv * per; g < end; ++g) s += (double)partial[(long long)g * n + i];
+    int g = slice;
+    for (; g + 96 < groups; g += 128) {  // four loads in flight
+      const float a = partial[(long long)g * n + i], b = partial[(long long)(g + 32) * n + i];
+      const float d = partial[(long long)(g + 64) * n + i], e = partial[(long long)(g + 96) * n + i];
+      s[0] += (double)a + (double)b;
+      s[1] += (double)d + (double)e;
+    }
+    for (; g < groups; g += 32) s[0] += (double)partial[(long long)g * n + i];
   }
-  part[wv][lane] = s;
+  part[slice][c] = s[0] + s[1];
   __syncthreads();
-  if (wv == 0 && i < n) {
-    s = 0.0;
+  if (slice == 0 && i < n) {
+    double t = 0.0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += part[k][lane];
-    (i < dim ? dw[i] : db[i - dim]) = (float)s;
+    for (int k = 0; k < 32; ++k) t += part[k][c];
+    (i < dim ? dw[i] : db[i - dim]) = (float)t;
   }
 }
 
@@ -408,7 +413,7 @@ int mia_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
   }
   if (dweight) {
     const int n = (int)(2 * dim);
-    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, s,
+    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s,
                        static_cast<const float*>(workspace), groups, n, dweight, dbias, (int)dim);
   }
   MIA_CHECK_HIP(hipGetLastError());

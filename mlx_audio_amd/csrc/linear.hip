@@ -2,32 +2,39 @@
 #include "linear_kernels.h"
 
 namespace mia {
-// out[i] = sum of the groups' partial sums in order, in double
+// out[i] = sum of the groups' partial sums in a fixed order, in double: 32 columns per workgroup, each of
+// its 32 slices every 32nd group
 __global__ __launch_bounds__(1024) void lin_bias_join_kernel(const float* __restrict__ partial, int groups, int n,
                                                             float* __restrict__ out) {
-  __shared__ double part[16][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int i = blockIdx.x * 64 + lane;
-  double s = 0.0;
+  __shared__ double part[32][32];
+  const int slice = threadIdx.x >> 5, c = threadIdx.x & 31;
+  const int i = blockIdx.x * 32 + c;
+  double s[2] = {};
   if (i < n) {
-    const int per = (groups + 15) / 16;
-    const int end = min(groups, (wv + 1) * per);
-    for (int g = wv * per; g < end; ++g) s += (double)partial[(long long)g * n + i];
+    int g = slice;
+    for (; g + 96 < groups; g += 128) {  // four loads in flight
+      const float a = partial[(long long)g * n + i], b = partial[(long long)(g + 32) * n + i];
+      const float d = partial[(long long)(g + 64) * n + i], e = partial[(long long)(g + 96) * n + i];
+      s[0] += (double)a + (double)b;
+      s[1] += (double)d + (double)e;
+    }
+    for (; g < groups; g += 32) s[0] += (double)partial[(long long)g * n + i];
   }
-  part[wv][lane] = s;
+  part[slice][c] = s[0] + s[1];
   __syncthreads();
-  if (wv == 0 && i < n) {
-    s = 0.0;
+  if (slice == 0 && i < n) {
+    double t = 0.0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += part[k][lane];
-    out[i] = (float)s;
+    for (int k = 0; k < 32; ++k) t += part[k][c];
+    out[i] = (float)t;
   }
 }
 
 namespace lin {
 constexpr long long kMaxSize = (1LL << 30) - 4096;  // positions along k are counted in 32 bits
 constexpr int kBiasGroups = 256;
-static int bias_groups(long long m) { return (int)((m + 3) / 4 < kBiasGroups ? (m + 3) / 4 : kBiasGroups); }
+// at least sixteen rows each
+static int bias_groups(long long m) { return (int)((m + 15) / 16 < kBiasGroups ? (m + 15) / 16 : kBiasGroups); }
 
 static int check(long long m, long long n, long long k, int dtype) {
   MIA_REQUIRE(m >= 0 && n >= 1 && k >= 1, "rows must be >= 0 and both widths >= 1 (got %lld rows, %lld -> %lld)", m, k, n);
@@ -123,7 +130,7 @@ int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_
       if (dz) g = dz, g_stride = out;
     }
     if (dbias) {
-      hipLaunchKernelGGL(lin_bias_join_kernel, dim3((unsigned)((out + 63) / 64)), dim3(1024), 0, s, sums, groups,
+      hipLaunchKernelGGL(lin_bias_join_kernel, dim3((unsigned)((out + 31) / 32)), dim3(1024), 0, s, sums, groups,
                          (int)out, dbias);
     }
     lin::Epilogue e{nullptr, 0, MIA_ACT_NONE, nullptr, 0, nullptr, nullptr};

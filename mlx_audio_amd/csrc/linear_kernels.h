@@ -518,8 +518,9 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
       });
     }
   } else {
-    u4 held[P];
-    auto fetch = [&](int step) {
+    // two stages ahead in registers: a stage is a fraction of memory's latency
+    u4 held[2][P];
+    auto fetch = [&](int step, u4(&to)[P]) {
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const bool isa = i < TL::PA, kc = isa ? AKC : BKC;
@@ -530,23 +531,28 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
         const int rows = isa ? p.n : p.m;
         const long long ld = isa ? p.lda : p.ldb;
         const T* base = static_cast<const T*>(isa ? p.a : p.b);
-        held[i] = u4{0, 0, 0, 0};
+        to[i] = u4{0, 0, 0, 0};
         if (row < rows && k < w.k_end)
-          held[i] = kc ? load_piece(base + row * ld + k, w.k_end - k) : load_piece(base + k * ld + row, rows - row);
+          to[i] = kc ? load_piece(base + row * ld + k, w.k_end - k) : load_piece(base + k * ld + row, rows - row);
       }
     };
-    if (steps > 0) fetch(0);
-    for (int s = 0; s < steps; ++s) {
+    auto stage_step = [&](int s, u4(&now)[P]) {
       unsigned char* stage = smem + (s & 1) * TL::STAGE;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const int at = i < TL::PA ? (TL::PA * wv + i) * 1024 : TL::A_BYTES + (TL::PB * wv + i - TL::PA) * 1024;
-        *reinterpret_cast<u4*>(stage + at + lane * 16) = held[i];
+        *reinterpret_cast<u4*>(stage + at + lane * 16) = now[i];
       }
       __syncthreads();  // this stage is written; every wave is done with the other one
-      if (s + 1 < steps) fetch(s + 1);
+      if (s + 2 < steps) fetch(s + 2, now);
       part.begin_stage(stage);
       part.run_stage(stage, [] {});
+    };
+    if (steps > 0) fetch(0, held[0]);
+    if (steps > 1) fetch(1, held[1]);
+    for (int s = 0; s < steps; s += 2) {
+      stage_step(s, held[0]);
+      if (s + 1 < steps) stage_step(s + 1, held[1]);
     }
   }
   part.store(p, w);
