@@ -167,7 +167,8 @@ struct Loader {
         where(i, wv, lane, r, c);
         held[i] = u4{0, 0, 0, 0};
         if (row0 + r < end && c * S::V < dim)
-          held[i] = load_piece(reinterpret_cast<const T*>(from) + r * stride + c * S::V, dim - c * S::V);
+          held[i] = load_piece(reinterpret_cast<const T*>(from) + r * stride + c * S::V, dim - c * S::V,
+                               (end - 1 - row0 - r) * stride + dim - c * S::V);
       }
     }
   }
@@ -182,15 +183,16 @@ struct Loader {
 // Keeps the compiler from doing a rare branch's selects always.
 __device__ __forceinline__ void rarely() { asm volatile(""); }
 
-// An own row's vector as the second operand: step cc, elements V (4 cc + (lane >> 4)) ...
+// An own row's vector as the second operand: step cc, elements V (4 cc + (lane >> 4)) ...; `behind`:
+// elements from the row's start to the start of the view's last row
 template <class T, int DP>
-__device__ __forceinline__ void load_own(const T* row, bool in, int dim, int lane, u4* out) {
+__device__ __forceinline__ void load_own(const T* row, bool in, int dim, long long behind, int lane, u4* out) {
   using S = Shape<T, DP>;
 #pragma unroll
   for (int cc = 0; cc < S::CC; ++cc) {
     const int e = (4 * cc + (lane >> 4)) * S::V;
     out[cc] = u4{0, 0, 0, 0};
-    if (in && e < dim) out[cc] = load_piece(row + e, dim - e);
+    if (in && e < dim) out[cc] = load_piece(row + e, dim - e, behind + dim - e);
   }
 }
 // An own column's results: 4 consecutive d of every accumulator per lane.
@@ -236,6 +238,19 @@ __device__ __forceinline__ bool order(unsigned pairs, unsigned per, unsigned& pa
 __device__ __forceinline__ int keys_of(const Args& p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.sk) : p.sk;
 }
+// The batch item of rank `r` by length, the longest first: work that ends last should be short.  (Up to
+// 64 items, one per lane; more, or no lengths: in order.)
+__device__ __forceinline__ int longest(const Args& p, int r) {
+  if (!p.lengths || p.batch > 64) return r;
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < p.batch ? p.lengths[lane] : -1;
+  int rank = 0;
+  for (int j = 0; j < p.batch; ++j) {
+    const int other = __builtin_amdgcn_readlane(mine, j);
+    rank += other > mine || (other == mine && j < lane) ? 1 : 0;
+  }
+  return __builtin_ctzll(__ballot(lane < p.batch && rank == r));
+}
 // sum / maximum over the four lanes that hold a column
 __device__ __forceinline__ float column_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -264,7 +279,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
   const int split = (int)(index % (unsigned)p.splits);
   // (causal: the last rows see most keys, so they start first)
   const int at_tile = (int)(index / (unsigned)p.splits), tile = p.causal ? p.own_tiles - 1 - at_tile : at_tile;
-  const int hg = (int)(pair % (unsigned)hgs), b = (int)(pair / (unsigned)hgs);
+  const int hg = (int)(pair % (unsigned)hgs), b = longest(p, (int)(pair / (unsigned)hgs));
   const int kvh = hg * p.pack / (p.heads / p.kv_heads);
   const int rows = p.sq * p.pack;
   const int row0 = tile * (64 * OT) + wv * (16 * OT);
@@ -287,8 +302,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
     const int r = row0 + 16 * o + (lane & 15);
     const bool in = r < rows;
     const int hl = in ? r / p.sq : 0, s = in ? r - hl * p.sq : 0;
-    load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + (hg * p.pack + hl) * p.q.h, in, p.dim, lane,
-                    own[o]);
+    load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + (hg * p.pack + hl) * p.q.h, in, p.dim,
+                    (p.sq - 1 - s) * p.q.s, lane, own[o]);
     limit[o] = p.causal ? min(len, s + off + 1) : len;
   }
   // every key before this one is seen by all of the wave's rows
@@ -477,7 +492,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   if (!order((unsigned)(p.batch * p.heads), (unsigned)(p.own_tiles * p.splits), pair, index)) return;
   const int split = (int)(index % (unsigned)p.splits), at_tile = (int)(index / (unsigned)p.splits);
   const int tile = p.causal ? p.own_tiles - 1 - at_tile : at_tile;
-  const int h = (int)(pair % (unsigned)p.heads), b = (int)(pair / (unsigned)p.heads);
+  const int h = (int)(pair % (unsigned)p.heads), b = longest(p, (int)(pair / (unsigned)p.heads));
   const int kvh = h / (p.heads / p.kv_heads);
   const int row0 = tile * (64 * OT) + wv * (16 * OT);
   const int off = p.sk - p.sq;
@@ -495,10 +510,13 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   for (int o = 0; o < OT; ++o) {
     const int s = row0 + 16 * o + (lane & 15);
     const bool in = s < p.sq;
-    load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + h * p.q.h, in, p.dim, lane, oq[o]);
-    load_own<T, DP>(static_cast<const T*>(p.dout.p) + b * p.dout.b + s * p.dout.s + h * p.dout.h, in, p.dim, lane, og[o]);
+    load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + h * p.q.h, in, p.dim,
+                    (p.sq - 1 - s) * p.q.s, lane, oq[o]);
+    load_own<T, DP>(static_cast<const T*>(p.dout.p) + b * p.dout.b + s * p.dout.s + h * p.dout.h, in, p.dim,
+                    (p.sq - 1 - s) * p.dout.s, lane, og[o]);
     u4 oo[S::CC];
-    load_own<T, DP>(static_cast<const T*>(p.out.p) + b * p.out.b + s * p.out.s + h * p.out.h, in, p.dim, lane, oo);
+    load_own<T, DP>(static_cast<const T*>(p.out.p) + b * p.out.b + s * p.out.s + h * p.out.h, in, p.dim,
+                    (p.sq - 1 - s) * p.out.s, lane, oo);
     float d = 0.0f;
 #pragma unroll
     for (int cc = 0; cc < S::CC; ++cc) {
@@ -636,8 +654,10 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
 #pragma unroll
   for (int o = 0; o < OT; ++o) {
     const int s = row0 + 16 * o + (lane & 15);
-    load_own<T, DP>(static_cast<const T*>(p.k.p) + b * p.k.b + (long long)s * p.k.s + kvh * p.k.h, s < len, p.dim, lane, ok[o]);
-    load_own<T, DP>(static_cast<const T*>(p.v.p) + b * p.v.b + (long long)s * p.v.s + kvh * p.v.h, s < len, p.dim, lane, ov[o]);
+    load_own<T, DP>(static_cast<const T*>(p.k.p) + b * p.k.b + (long long)s * p.k.s + kvh * p.k.h, s < len, p.dim,
+                    (p.sk - 1 - s) * p.k.s, lane, ok[o]);
+    load_own<T, DP>(static_cast<const T*>(p.v.p) + b * p.v.b + (long long)s * p.v.s + kvh * p.v.h, s < len, p.dim,
+                    (p.sk - 1 - s) * p.v.s, lane, ov[o]);
   }
   f4 dk[S::DT][OT], dv[S::DT][OT];
 #pragma unroll

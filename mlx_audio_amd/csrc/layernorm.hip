@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(ln::Args p) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = (c * LANES + t) * V;
-      unpack<T>(load_piece(x + i, dim - i), v + c * V);
+      unpack<T>(load_piece(x + i, dim - i, (p.rows - 1 - row) * p.x_stride + dim - i), v + c * V);
     }
     float s = 0.0f;
 #pragma unroll
@@ -140,8 +140,8 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(ln::Args p) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = (c * LANES + t) * V;
-      unpack<T>(load_piece(x + i, dim - i), h + c * V);
-      unpack<T>(load_piece(dy + i, dim - i), g + c * V);  // zero behind the row: no share in any sum
+      unpack<T>(load_piece(x + i, dim - i, (p.rows - 1 - row) * p.x_stride + dim - i), h + c * V);
+      unpack<T>(load_piece(dy + i, dim - i, (p.rows - 1 - row) * p.dy_stride + dim - i), g + c * V);  // zero behind the row: no share in any sum
     }
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll

@@ -533,7 +533,8 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
         const T* base = static_cast<const T*>(isa ? p.a : p.b);
         to[i] = u4{0, 0, 0, 0};
         if (row < rows && k < w.k_end)
-          to[i] = kc ? load_piece(base + row * ld + k, w.k_end - k) : load_piece(base + k * ld + row, rows - row);
+          to[i] = kc ? load_piece(base + row * ld + k, w.k_end - k, (rows - 1 - row) * ld + p.k - k)
+                     : load_piece(base + k * ld + row, rows - row, (p.k - 1 - k) * ld + rows - row);
       }
     };
     auto stage_step = [&](int s, u4(&now)[P]) {
@@ -687,9 +688,9 @@ __global__ __launch_bounds__(64 * NW) void lin_few_kernel(lin::Gemm p) {
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int k = k0 + u * NW * KSTEP + g * V;
-      fa[u] = load_piece(a + k, n_in ? p.k - k : 0);
+      fa[u] = load_piece(a + k, n_in ? p.k - k : 0, (p.n - 1 - n0 - r15) * p.lda + p.k - k);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) fb[u][j] = load_piece(b[j] + k, m_in[j] ? p.k - k : 0);
+      for (int j = 0; j < MT; ++j) fb[u][j] = load_piece(b[j] + k, m_in[j] ? p.k - k : 0, (p.m - 1 - 16 * j - r15) * p.ldb + p.k - k);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
@@ -737,10 +738,10 @@ __global__ __launch_bounds__(256) void lin_dz_kernel(const T* __restrict__ dy, l
   if (left > 0) {
     for (long long row = (long long)blockIdx.y * 4 + wv; row < m; row += (long long)gridDim.y * 4) {
       float g[V];
-      unpack<T>(load_piece(dy + row * dy_stride + c0, left), g);
+      unpack<T>(load_piece(dy + row * dy_stride + c0, left, (m - 1 - row) * dy_stride + left), g);
       if (z) {
         float zz[V];
-        unpack<T>(load_piece(z + row * z_stride + c0, left), zz);
+        unpack<T>(load_piece(z + row * z_stride + c0, left, (m - 1 - row) * z_stride + left), zz);
 #pragma unroll
         for (int j = 0; j < V; ++j) g[j] *= derivative<sizeof(T) == 4>(zz[j], act);
         store_piece(dz + row * n + c0, pack<T>(g), left);

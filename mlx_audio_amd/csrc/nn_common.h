@@ -24,20 +24,33 @@ struct __attribute__((packed, aligned(2))) Raw16 {
 template <class T>
 constexpr int kPer16 = 16 / (int)sizeof(T);
 
-// elements [0, n) of the 16-byte piece at p, zeros behind; n may be <= 0
+// Elements [0, n) of the 16-byte piece at p, zeros behind; n may be <= 0.  `room`: elements from p on that
+// belong to the same array (its later rows): where that is a whole piece, a row's end costs one load and
+// three masks; element by element (each a load of its own) only at the array's very end.
 template <class T>
-__device__ __forceinline__ u4 load_piece(const T* p, int n) {
+__device__ __forceinline__ u4 load_piece(const T* p, int n, long long room = 0) {
   constexpr int V = kPer16<T>;
   if (n >= V) return reinterpret_cast<const Raw16*>(p)->v;
+  u4 x = u4{0, 0, 0, 0};
+  if (n <= 0) return x;
+  if (room >= V) {
+    x = reinterpret_cast<const Raw16*>(p)->v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int bytes = n * (int)sizeof(T) - 4 * j;  // of this word inside
+      x[j] = bytes >= 4 ? x[j] : bytes == 2 ? x[j] & 0xffffu : 0u;
+    }
+    return x;
+  }
   union {
     u4 u;
     T e[V];
-  } x;
-  x.u = u4{0, 0, 0, 0};
+  } y;
+  y.u = x;
 #pragma unroll
   for (int j = 0; j < V - 1; ++j)
-    if (j < n) x.e[j] = p[j];
-  return x.u;
+    if (j < n) y.e[j] = p[j];
+  return y.u;
 }
 template <class T>
 __device__ __forceinline__ void store_piece(T* p, u4 v, int n) {
