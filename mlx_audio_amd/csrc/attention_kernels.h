@@ -576,7 +576,10 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
 #pragma unroll
       for (int r = 0; r < S::RB; ++r)
 #pragma unroll
-        for (int o = 0; o < OT; ++o) s[r][o] = dp[r][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int o = 0; o < OT; ++o) {  // dp begins at -delta: it is only used less delta
+          s[r][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+          dp[r][o] = f4{-delta[o], -delta[o], -delta[o], -delta[o]};
+        }
 #pragma unroll
       for (int cc = 0; cc < S::CC; ++cc)
 #pragma unroll
@@ -607,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
         for (int r = 0; r < S::RB; ++r)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            blocks[r][i] = exp2_fast(fmaf(s[r][o][i], c, -lse2[o])) * (dp[r][o][i] - delta[o]);
+            blocks[r][i] = exp2_fast(fmaf(s[r][o][i], c, -lse2[o])) * dp[r][o][i];
           }
         df[o] = to_operand<T>(blocks);
       }
@@ -701,32 +704,43 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     if (t + 1 < end) issue(t + 1);
     if (row0 >= len) continue;
     const bool masked = row0 + 16 * OT > len || (p.causal && row0 + 16 * OT - 1 > q0 + off);
-#pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      f4 s[S::RB][OT], dp[S::RB][OT];
-#pragma unroll
-      for (int r = 0; r < S::RB; ++r)
-#pragma unroll
-        for (int o = 0; o < OT; ++o) s[r][o] = dp[r][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int cc = 0; cc < S::CC; ++cc)
-#pragma unroll
-        for (int r = 0; r < S::RB; ++r) {
-          const u4 fq = rows_fragment<T, DP>(qt, st * S::RB + r, cc, lane);
-          const u4 fg = rows_fragment<T, DP>(gt, st * S::RB + r, cc, lane);
-#pragma unroll
-          for (int o = 0; o < OT; ++o) {
-            s[r][o] = Mma<T>::step(fq, ok[o][cc], s[r][o]);
-            dp[r][o] = Mma<T>::step(fg, ov[o][cc], dp[r][o]);
-          }
-        }
-      f4 lse2[S::RB], delta[S::RB];
+    // the row fragments of a step are read while the step before it works on its products
+    u4 rq[S::RB][S::CC], rg[S::RB][S::CC];
+    f4 lse2[S::RB], delta[S::RB];
+    auto read_rows = [&](int st) {
 #pragma unroll
       for (int r = 0; r < S::RB; ++r) {
         const int at = 16 * (st * S::RB + r) + 4 * g;
         lse2[r] = *reinterpret_cast<const f4*>(&rows_lse[t & 1][at]);
         delta[r] = *reinterpret_cast<const f4*>(&rows_delta[t & 1][at]);
+#pragma unroll
+        for (int cc = 0; cc < S::CC; ++cc) {
+          rq[r][cc] = rows_fragment<T, DP>(qt, st * S::RB + r, cc, lane);
+          rg[r][cc] = rows_fragment<T, DP>(gt, st * S::RB + r, cc, lane);
+        }
       }
+    };
+    read_rows(0);
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      f4 s[S::RB][OT], dp[S::RB][OT];  // dp begins at -delta: it is only used less delta
+#pragma unroll
+      for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+        for (int o = 0; o < OT; ++o) s[r][o] = f4{0.0f, 0.0f, 0.0f, 0.0f}, dp[r][o] = -delta[r];
+#pragma unroll
+      for (int cc = 0; cc < S::CC; ++cc)
+#pragma unroll
+        for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+          for (int o = 0; o < OT; ++o) {
+            s[r][o] = Mma<T>::step(rq[r][cc], ok[o][cc], s[r][o]);
+            dp[r][o] = Mma<T>::step(rg[r][cc], ov[o][cc], dp[r][o]);
+          }
+      f4 minus[S::RB];
+#pragma unroll
+      for (int r = 0; r < S::RB; ++r) minus[r] = -lse2[r];
+      if (st + 1 < STEPS) read_rows(st + 1);
       if (masked) {
         rarely();
 #pragma unroll
@@ -749,9 +763,9 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
         for (int r = 0; r < S::RB; ++r)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e = exp2_fast(fmaf(s[r][o][i], c, -lse2[r][i]));
+            const float e = exp2_fast(fmaf(s[r][o][i], c, minus[r][i]));
             pb[r][i] = e;
-            db[r][i] = e * (dp[r][o][i] - delta[r][i]);
+            db[r][i] = e * dp[r][o][i];
           }
         pf[o] = to_operand<T>(pb);
         df[o] = to_operand<T>(db);
