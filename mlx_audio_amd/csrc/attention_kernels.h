@@ -76,23 +76,38 @@ __device__ __forceinline__ int turn(int r) {
   if (DP <= 64) return (r & 6) | ((r >> 3) & 1);
   return ((r & 7) << 1) | ((r >> 3) & 1);
 }
+// A lane's place in LDS for either kind of read of a tile that starts at byte `tile` (a multiple of 1024),
+// worked out once: every other address is it, with bits above the bank turned (^) and constants added.
+template <class T, int DP>
+__device__ __forceinline__ unsigned rows_place(unsigned tile, int lane) {
+  const int row = lane & 15, g = lane >> 4;
+  return tile + row * Shape<T, DP>::PITCH + ((g ^ turn<T, DP>(row)) << 4);
+}
+template <class T, int DP>
+__device__ __forceinline__ unsigned columns_place(unsigned tile, int lane) {
+  using S = Shape<T, DP>;
+  const int r = lane & 15, g = lane >> 4;
+  if constexpr (S::ES == 2) {
+    const int row = 4 * g + (r >> 2);
+    return tile + row * S::PITCH + ((((r & 3) >> 1) ^ turn<T, DP>(row)) << 4) + 8 * (r & 1);
+  } else {
+    return tile + 4 * g * S::PITCH + (((r >> 2) ^ turn<T, DP>(4 * g)) << 4) + 4 * (r & 3);
+  }
+}
+typedef const __attribute__((address_space(3))) u4* lds_u4;
+typedef const __attribute__((address_space(3))) unsigned* lds_u1;
 // 16 bytes of 16 rows: row block `rb`, piece 4 cc + (lane >> 4)
 template <class T, int DP>
-__device__ __forceinline__ u4 rows_fragment(const unsigned char* tile, int rb, int cc, int lane) {
-  using S = Shape<T, DP>;
-  const int row = 16 * rb + (lane & 15), c = 4 * cc + (lane >> 4);
-  return *reinterpret_cast<const u4*>(tile + row * S::PITCH + ((c ^ turn<T, DP>(row)) << 4));
+__device__ __forceinline__ u4 rows_fragment(unsigned place, int rb, int cc) {
+  return *(lds_u4)(unsigned long long)((place ^ (cc << 6)) + rb * 16 * Shape<T, DP>::PITCH);
 }
 // Columns: lane's column is d = 16 dt + (lane & 15), its elements are the stream rows of step `st` in
 // the order of the product tiles: rows 4 (lane >> 4) + i of each 16-row block.
 template <class T, int DP>
-__device__ __forceinline__ u4 columns_fragment(const unsigned char* tile, int st, int dt, int lane) {
+__device__ __forceinline__ u4 columns_fragment(unsigned place, int st, int dt) {
   using S = Shape<T, DP>;
-  const int r = lane & 15, g = lane >> 4;
   if constexpr (S::ES == 2) {
-    const int row = 32 * st + 4 * g + (r >> 2), d = 16 * dt + 4 * (r & 3);
-    const unsigned at =
-        (unsigned)(unsigned long long)tile + row * S::PITCH + (((d >> 3) ^ turn<T, DP>(row)) << 4) + (d & 7) * 2;
+    const unsigned at = (place ^ (dt << 5)) + st * 32 * S::PITCH;
     union {
       s4 h[2];
       u4 u;
@@ -101,13 +116,10 @@ __device__ __forceinline__ u4 columns_fragment(const unsigned char* tile, int st
     x.h[1] = lds_read_column4(at + 16 * S::PITCH);
     return x.u;
   } else {
-    const int d = 16 * dt + r;
     u4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 16 * st + 4 * g + i;
-      x[i] = *reinterpret_cast<const unsigned*>(tile + row * S::PITCH + (((d >> 2) ^ turn<T, DP>(row)) << 4) + (d & 3) * 4);
-    }
+    for (int i = 0; i < 4; ++i)
+      x[i] = *(lds_u1)(unsigned long long)((place ^ ((dt << 6) | (i << 4))) + (16 * st + i) * S::PITCH);
     return x;
   }
 }
@@ -269,7 +281,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
   using namespace att;
   using S = Shape<T, DP>;
   constexpr int KB = S::TILE / 16, STEPS = KB / S::RB;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * S::BYTES];  // two buffers of k and v
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * S::BYTES];  // two buffers of k and v
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
 
@@ -281,7 +293,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
   const int at_tile = (int)(index / (unsigned)p.splits), tile = p.causal ? p.own_tiles - 1 - at_tile : at_tile;
   const int hg = (int)(pair % (unsigned)hgs), b = longest(p, (int)(pair / (unsigned)hgs));
   const int kvh = hg * p.pack / (p.heads / p.kv_heads);
-  const int rows = p.sq * p.pack;
+  const int all_rows = p.sq * p.pack;
   const int row0 = tile * (64 * OT) + wv * (16 * OT);
   const int off = p.sk - p.sq;
   const float c = p.scale * kLog2e;
@@ -289,7 +301,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
   int len = keys_of(p, b);
   int k_begin = split * p.keys_per_split;
   int k_end = min(len, k_begin + p.keys_per_split);
-  const int first_row = tile * (64 * OT), last_row = min(rows, first_row + 64 * OT) - 1;
+  const int first_row = tile * (64 * OT), last_row = min(all_rows, first_row + 64 * OT) - 1;
   if (p.causal) {  // the furthest key that a row of this workgroup sees
     const int far = first_row / p.sq == last_row / p.sq ? last_row % p.sq : p.sq - 1;
     k_end = min(k_end, far + off + 1);
@@ -300,7 +312,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
 #pragma unroll
   for (int o = 0; o < OT; ++o) {
     const int r = row0 + 16 * o + (lane & 15);
-    const bool in = r < rows;
+    const bool in = r < all_rows;
     const int hl = in ? r / p.sq : 0, s = in ? r - hl * p.sq : 0;
     load_own<T, DP>(static_cast<const T*>(p.q.p) + b * p.q.b + s * p.q.s + (hg * p.pack + hl) * p.q.h, in, p.dim,
                     (p.sq - 1 - s) * p.q.s, lane, own[o]);
@@ -309,8 +321,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
   // every key before this one is seen by all of the wave's rows
   int open = len;
   if (p.causal) {
-    const int last = min(rows, row0 + 16 * OT) - 1;
-    const int near = row0 < rows && row0 / p.sq == last / p.sq ? row0 % p.sq : 0;
+    const int last = min(all_rows, row0 + 16 * OT) - 1;
+    const int near = row0 < all_rows && row0 / p.sq == last / p.sq ? row0 % p.sq : 0;
     open = min(len, near + off + 1);
   }
 
@@ -326,6 +338,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
   const T* kp = static_cast<const T*>(p.k.p) + b * p.k.b + kvh * p.k.h;
   const T* vp = static_cast<const T*>(p.v.p) + b * p.v.b + kvh * p.v.h;
   const unsigned lds0 = (unsigned)(unsigned long long)smem;
+  const unsigned rows0 = rows_place<T, DP>(lds0, lane), columns0 = columns_place<T, DP>(lds0, lane);
   Loader<T, DP, DMA> lk, lv;
   lk.init(p.k.s, p.dim, wv, lane);
   lv.init(p.v.s, p.dim, wv, lane);
@@ -341,13 +354,14 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
     lv.commit(vt, wv, lane);
     wait_loads<0>();
     barrier_keep_loads();  // tile t is there, and nobody reads the other buffer any more
+    const unsigned rows = rows0 + (t & 1) * 2 * S::BYTES, columns = columns0 + (t & 1) * 2 * S::BYTES;
     const int k0 = k_begin + t * S::TILE;
     if (t + 1 < tiles) {
       const unsigned next = lds0 + ((t + 1) & 1) * 2 * S::BYTES;
       lk.issue(kp, p.k.s, k0 + S::TILE, k_end, p.dim, next, wv, lane);
       lv.issue(vp, p.v.s, k0 + S::TILE, k_end, p.dim, next + S::BYTES, wv, lane);
     }
-    if (row0 >= rows) continue;
+    if (row0 >= all_rows) continue;
 
     f4 s[KB][OT];
 #pragma unroll
@@ -358,7 +372,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
     for (int cc = 0; cc < S::CC; ++cc)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const u4 f = rows_fragment<T, DP>(kt, kb, cc, lane);
+        const u4 f = rows_fragment<T, DP>(rows, kb, cc);
 #pragma unroll
         for (int o = 0; o < OT; ++o) s[kb][o] = Mma<T>::step(f, own[o][cc], s[kb][o]);
       }
@@ -415,7 +429,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
       }
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) {
-        const u4 f = columns_fragment<T, DP>(vt, st, d, lane);
+        const u4 f = columns_fragment<T, DP>(columns + S::BYTES, st, d);
 #pragma unroll
         for (int o = 0; o < OT; ++o) acc[d][o] = Mma<T>::step(f, pf[o], acc[d][o]);
       }
@@ -425,7 +439,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
 #pragma unroll
   for (int o = 0; o < OT; ++o) {
     const int r = row0 + 16 * o + (lane & 15);
-    if (r >= rows) continue;   // (its other three lanes leave too)
+    if (r >= all_rows) continue;   // (its other three lanes leave too)
     const float total = column_sum(sum[o]);
     const int hl = r / p.sq, s = r - hl * p.sq, h = hg * p.pack + hl;
     const long long at = ((long long)b * p.heads + h) * p.sq + s;
@@ -485,7 +499,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   using namespace att;
   using S = Shape<T, DP>;
   constexpr int STEPS = S::TILE / 16 / S::RB;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * S::BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * S::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
   unsigned pair, index;
@@ -545,6 +559,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   const T* kp = static_cast<const T*>(p.k.p) + b * p.k.b + kvh * p.k.h;
   const T* vp = static_cast<const T*>(p.v.p) + b * p.v.b + kvh * p.v.h;
   const unsigned lds0 = (unsigned)(unsigned long long)smem;
+  const unsigned rows0 = rows_place<T, DP>(lds0, lane), columns0 = columns_place<T, DP>(lds0, lane);
   Loader<T, DP, DMA> lk, lv;
   lk.init(p.k.s, p.dim, wv, lane);
   lv.init(p.v.s, p.dim, wv, lane);
@@ -562,6 +577,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
     lv.commit(vt, wv, lane);
     wait_loads<0>();
     barrier_keep_loads();
+    const unsigned rows = rows0 + (t & 1) * 2 * S::BYTES, columns = columns0 + (t & 1) * 2 * S::BYTES;
     const int k0 = t * S::TILE;
     if (t + 1 < end) {
       const unsigned next = lds0 + ((t + 1) & 1) * 2 * S::BYTES;
@@ -584,8 +600,8 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
       for (int cc = 0; cc < S::CC; ++cc)
 #pragma unroll
         for (int r = 0; r < S::RB; ++r) {
-          const u4 fk = rows_fragment<T, DP>(kt, st * S::RB + r, cc, lane);
-          const u4 fv = rows_fragment<T, DP>(vt, st * S::RB + r, cc, lane);
+          const u4 fk = rows_fragment<T, DP>(rows, st * S::RB + r, cc);
+          const u4 fv = rows_fragment<T, DP>(rows + S::BYTES, st * S::RB + r, cc);
 #pragma unroll
           for (int o = 0; o < OT; ++o) {
             s[r][o] = Mma<T>::step(fk, oq[o][cc], s[r][o]);
@@ -616,7 +632,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
       }
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) {
-        const u4 f = columns_fragment<T, DP>(kt, st, d, lane);
+        const u4 f = columns_fragment<T, DP>(columns, st, d);
 #pragma unroll
         for (int o = 0; o < OT; ++o) acc[d][o] = Mma<T>::step(f, df[o], acc[d][o]);
       }
@@ -638,7 +654,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   using namespace att;
   using S = Shape<T, DP>;
   constexpr int STEPS = S::TILE / 16 / S::RB;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * S::BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * S::BYTES];
   __shared__ float rows_lse[2][64], rows_delta[2][64];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4;
@@ -675,6 +691,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   const int begin = (int)((long long)all * split / p.splits), end = (int)((long long)all * (split + 1) / p.splits);
   const long long n = (long long)p.batch * p.heads * p.sq;
   const unsigned lds0 = (unsigned)(unsigned long long)smem;
+  const unsigned rows0 = rows_place<T, DP>(lds0, lane), columns0 = columns_place<T, DP>(lds0, lane);
   const unsigned lse_at = (unsigned)(unsigned long long)&rows_lse[0][0];
   const unsigned delta_at = (unsigned)(unsigned long long)&rows_delta[0][0];
   Loader<T, DP, DMA> lq, lg;
@@ -700,6 +717,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     lg.commit(gt, wv, lane);
     wait_loads<0>();
     barrier_keep_loads();
+    const unsigned rows = rows0 + (t & 1) * 2 * S::BYTES, columns = columns0 + (t & 1) * 2 * S::BYTES;
     const int q0 = first + t % per_head * S::TILE;
     if (t + 1 < end) issue(t + 1);
     if (row0 >= len) continue;
@@ -715,8 +733,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
         delta[r] = *reinterpret_cast<const f4*>(&rows_delta[t & 1][at]);
 #pragma unroll
         for (int cc = 0; cc < S::CC; ++cc) {
-          rq[r][cc] = rows_fragment<T, DP>(qt, st * S::RB + r, cc, lane);
-          rg[r][cc] = rows_fragment<T, DP>(gt, st * S::RB + r, cc, lane);
+          rq[r][cc] = rows_fragment<T, DP>(rows, st * S::RB + r, cc);
+          rg[r][cc] = rows_fragment<T, DP>(rows + S::BYTES, st * S::RB + r, cc);
         }
       }
     };
@@ -772,8 +790,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
       }
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) {
-        const u4 fg = columns_fragment<T, DP>(gt, st, d, lane);
-        const u4 fq = columns_fragment<T, DP>(qt, st, d, lane);
+        const u4 fg = columns_fragment<T, DP>(columns + S::BYTES, st, d);
+        const u4 fq = columns_fragment<T, DP>(columns, st, d);
 #pragma unroll
         for (int o = 0; o < OT; ++o) {
           dv[d][o] = Mma<T>::step(fg, pf[o], dv[d][o]);
