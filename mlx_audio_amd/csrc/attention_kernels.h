@@ -263,10 +263,12 @@ __device__ __forceinline__ int longest(const Args& p, int r) {
   }
   return __builtin_ctzll(__ballot(lane < p.batch && rank == r));
 }
+// one v_maximum3_f32 for two of them (fmaxf quiets its operands first); a NaN stays one
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // sum / maximum over the four lanes that hold a column
 __device__ __forceinline__ float column_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  v = maximum(v, __shfl_xor(v, 16));
+  return maximum(v, __shfl_xor(v, 32));
 }
 __device__ __forceinline__ float column_sum(float v) {
   v += __shfl_xor(v, 16);
@@ -392,7 +394,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, s[kb][o][i]);
+        for (int i = 0; i < 4; ++i) m = maximum(m, s[kb][o][i]);
       // The reference that exponents are taken against follows the running maximum only when that is
       // more than 8 above it: p then stays below 2^8 (far from any type's limit; a sum's precision does
       // not depend on it), and after the first tiles nothing is rescaled any more.
