@@ -818,14 +818,15 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   }
 }
 
-// A gradient's parts added in order: out[i] = sum over splits of partial[split * stride + i].
+// Gradients' parts added in order: out[i] = sum over splits of partial[split * total + i], i < total; the
+// first n go to out0, the rest to out1.
 template <class T>
-__global__ __launch_bounds__(256) void att_add_kernel(const float* __restrict__ partial, long long stride, int splits,
-                                                      long long n, T* __restrict__ out) {
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void att_add_kernel(const float* __restrict__ partial, long long total, int splits,
+                                                      long long n, T* __restrict__ out0, T* __restrict__ out1) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     float v = partial[i];
-    for (int s = 1; s < splits; ++s) v += partial[s * stride + i];
-    out[i] = (T)v;
+    for (int s = 1; s < splits; ++s) v += partial[s * total + i];
+    (i < n ? out0[i] : out1[i - n]) = (T)v;
   }
 }
 
@@ -937,10 +938,10 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
   const bool whole = a.dim % (16 / (int)sizeof(T)) == 0;
   a.stats = stats, a.pack = 1;
   a.partial = stats + align256((size_t)2 * rows * sizeof(float)) / sizeof(float);
-  auto add = [&](const float* partial, long long stride, long long n, void* out) {
-    const long long blocks = (n + 255) / 256;
-    hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, partial,
-                       stride, a.splits, n, static_cast<T*>(out));
+  auto add = [&](long long total, long long n, void* out0, void* out1) {
+    const long long blocks = (total + 255) / 256;
+    hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a.partial,
+                       total, a.splits, n, static_cast<T*>(out0), static_cast<T*>(out1));
   };
   if (rows) {
     const GradPlan pl = plan_dq(a.batch, a.sq, a.sk, a.heads, sizeof(T));
@@ -951,7 +952,7 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
       if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_dq_kernel, 2, grid);
       else MIA_ATT_LAUNCH(att_dq_kernel, 1, grid);
     });
-    if (a.splits > 1) add(a.partial, rows * a.dim, rows * a.dim, dq);
+    if (a.splits > 1) add(rows * a.dim, rows * a.dim, dq, nullptr);
   }
   if (a.sk) {
     const GradPlan pl = plan_dkv(a.batch, a.sq, a.sk, a.heads, a.kv_heads, a.dim, sizeof(T));
@@ -972,8 +973,7 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
     });
     if (a.splits > 1) {
       const long long n = (long long)a.batch * a.sk * a.kv_heads * a.dim;
-      add(a.partial, 2 * n, n, dk);
-      add(a.partial + n, 2 * n, n, dv);
+      add(2 * n, n, dk, dv);
     }
   }
   return MIA_OK;

@@ -105,7 +105,10 @@ __device__ __forceinline__ void finish(T* out, T* z, int left, const float* b, u
   constexpr bool PRECISE = sizeof(T) == 4;
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] += b[j];
-  if (z) store_piece(z, pack<T>(v), left);
+  // z is read by a backward pass, long after: past the caches.  (24000 x 1280 -> 5120, bfloat16, GELU: 412 ->
+  // 399 us.  The result itself stays in them, though 386 us would do without: what follows reads it, and
+  // a block of the encoder on 8 - 16 clips took 2 - 3 % longer then.)
+  if (z) store_piece<T, true>(z, pack<T>(v), left);
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] = activate<PRECISE>(v[j], ACT);
   if constexpr (PLUS) {
@@ -807,6 +810,7 @@ static Choice choose(long long n, long long m, long long k, size_t es, bool dma,
       const long long groups = tiles * splits, per_cu = (groups + kCus - 1) / kCus;
       const double load = per_cu < kd.per_cu ? (double)per_cu / kd.per_cu : 1.0;  // a stage is faster alone
       double stage = (es == 4 ? kd.stage4 : kd.stage2) * (0.45 + 0.55 * load);
+      if (!dma) stage *= kd.tile == 64 ? 1.6 : columns ? 3.4 : 1.9;  // pieces through registers
       if (kd.tile == 256) stage = es == 4 ? (columns ? 11.0 : kd.stage4) : (columns ? 1.8 : kd.stage2);
       const long long rounds = (groups + (long long)kCus * kd.per_cu - 1) / ((long long)kCus * kd.per_cu);
       double t = (double)rounds * ((double)((steps + splits - 1) / splits) * stage + kd.ends);

@@ -52,11 +52,14 @@ __device__ __forceinline__ u4 load_piece(const T* p, int n, long long room = 0) 
     if (j < n) y.e[j] = p[j];
   return y.u;
 }
-template <class T>
+// PAST: the result goes past the caches (a nontemporal store).
+template <class T, bool PAST = false>
 __device__ __forceinline__ void store_piece(T* p, u4 v, int n) {
   constexpr int V = kPer16<T>;
   if (n >= V) {
-    reinterpret_cast<Raw16*>(p)->v = v;
+    typedef u4 __attribute__((aligned(2))) u4a;
+    if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<u4a*>(p));
+    else reinterpret_cast<Raw16*>(p)->v = v;
     return;
   }
   union {
@@ -182,7 +185,6 @@ static inline bool dtype_ok(int d) { return d == MIA_F32 || d == MIA_F16 || d ==
 static inline size_t dtype_size(int d) { return d == MIA_F32 ? 4 : 2; }
 static inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-static inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // Calls f(T()) with the element type that `dtype` names.
 template <class F>

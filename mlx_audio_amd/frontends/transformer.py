@@ -99,7 +99,7 @@ def _ptr(x):
 def _check_vector(x, name: str, n: int, dtype: torch.dtype) -> None:
     if x is None:
         return
-    if tuple(x.shape) != (n,):
+    if x.shape != (n,):
         raise ValueError(f"{name} must have shape ({n},), got {tuple(x.shape)}")
     if x.dtype not in (dtype, torch.float32):
         raise ValueError(f"{name} must be float32 or {dtype}, got {x.dtype}")
@@ -130,12 +130,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool 
     w = None if w is None else w.contiguous()
     b = None if b is None else b.contiguous()
     flat, rows, stride = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
     if return_stats:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+        mean = flat.new_empty(x.shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
-    params = next((v for v in (w, b) if v is not None), flat)
+    params = w if w is not None else b if b is not None else flat
     _call(_lib.lib().mia_layer_norm, device, flat.data_ptr(), rows, x.shape[-1], stride, _DTYPES[x.dtype], _ptr(w),
           _ptr(b), _DTYPES[params.dtype], float(eps), y.data_ptr(), _ptr(mean) if rows else None,
           _ptr(rstd) if rows else None)
@@ -165,15 +165,15 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     mean, rstd = ops["mean"].contiguous(), ops["rstd"].contiguous()
     w = None if weight is None else ops["weight"].contiguous()
     dim = x.shape[-1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    dx = flat.new_empty(x.shape)
     dw = db = ws = None
     lib = _lib.lib()
     need = 0
     if w is not None:
-        dw = torch.empty((dim,), dtype=torch.float32, device=device)
+        dw = flat.new_empty((dim,), dtype=torch.float32)
         db = torch.empty_like(dw)
         need = lib.mia_layer_norm_backward_workspace_bytes(rows, dim)
-        ws = torch.empty((need,), dtype=torch.uint8, device=device)
+        ws = flat.new_empty((need,), dtype=torch.uint8)
     _call(lib.mia_layer_norm_backward, device, gflat.data_ptr(), gstride, flat.data_ptr(), stride, mean.data_ptr(),
           rstd.data_ptr(), rows, dim, _DTYPES[x.dtype], _ptr(w), _DTYPES[(flat if w is None else w).dtype],
           dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), need)
@@ -214,11 +214,11 @@ def linear(x, weight, bias=None, activation=None, residual=None, return_preactiv
     r, rstride = None, 0
     if residual is not None:
         r, _, rstride = _rows(ops["residual"])
-    y = torch.empty(shape, dtype=dtype, device=device)
+    y = flat.new_empty(shape)
     z = torch.empty_like(y) if return_preactivation else None
     lib = _lib.lib()
     need = lib.mia_linear_workspace_bytes(rows, k, n, _DTYPES[dtype])
-    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    ws = flat.new_empty((need,), dtype=torch.uint8) if need else None
     _call(lib.mia_linear, device, flat.data_ptr(), stride, w.data_ptr(), wstride, _ptr(b),
           _DTYPES[(flat if b is None else b).dtype], _ptr(r), rstride, _ACTIVATIONS[activation], rows, k, n,
           _DTYPES[dtype], y.data_ptr(), _ptr(z), _ptr(ws), need)
@@ -255,13 +255,13 @@ def linear_backward(dy, x, weight, activation=None, preactivation=None, input_gr
     zf, zstride = None, 0
     if activation is not None:
         zf, _, zstride = _rows(ops["preactivation"])
-    dx = torch.empty(x.shape, dtype=dtype, device=device) if input_grad else None
-    dw = torch.empty((n, k), dtype=dtype, device=device) if weight_grad else None
-    db = torch.empty((n,), dtype=torch.float32, device=device) if bias_grad else None
+    dx = flat.new_empty(x.shape) if input_grad else None
+    dw = flat.new_empty((n, k)) if weight_grad else None
+    db = flat.new_empty((n,), dtype=torch.float32) if bias_grad else None
     lib = _lib.lib()
     act = _ACTIVATIONS[activation]
     need = lib.mia_linear_backward_workspace_bytes(rows, k, n, _DTYPES[dtype], act)
-    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    ws = flat.new_empty((need,), dtype=torch.uint8) if need else None
     _call(lib.mia_linear_backward, device, g.data_ptr(), gstride, flat.data_ptr(), stride, w.data_ptr(), wstride,
           _ptr(zf), zstride, act, rows, k, n, _DTYPES[dtype], _ptr(dx) if rows else None, _ptr(dw), _ptr(db), _ptr(ws),
           need)
@@ -307,7 +307,8 @@ def _heads(x: torch.Tensor) -> torch.Tensor:
 
 
 def _strides(x: torch.Tensor):
-    return (ctypes.c_int64 * 3)(*x.stride()[:3])
+    # (an axis of one element may have any stride)
+    return (ctypes.c_int64 * 3)(*(st if n > 1 else 0 for n, st in zip(x.shape, x.stride()[:3])))
 
 
 def _attention_desc(q, k, v, causal, scale) -> _lib.AttentionDesc:
@@ -339,12 +340,12 @@ def attention(q, k, v, causal: bool = False, key_lengths=None, scale=None, retur
     device = _to_device(ops)
     q, k, v = (_heads(ops[n]) for n in ("q", "k", "v"))
     lengths = ops.get("key_lengths")
-    out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=device)
-    lse = torch.empty((B, H, Sq), dtype=torch.float32, device=device) if return_lse else None
+    out = q.new_empty((B, Sq, H, D))
+    lse = q.new_empty((B, H, Sq), dtype=torch.float32) if return_lse else None
     desc = _attention_desc(q, k, v, causal, scale)
     lib = _lib.lib()
     need = lib.mia_attention_workspace_bytes(ctypes.byref(desc))
-    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _call(lib.mia_attention, device, ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths),
           out.data_ptr(), _ptr(lse), _ptr(ws), need)
     return (out, lse) if return_lse else out
@@ -372,13 +373,11 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool = False, key_length
     device = _to_device(ops)
     dout, q, k, v, out = (_heads(ops[n]) for n in ("dout", "q", "k", "v", "out"))
     lse, lengths = ops["lse"].contiguous(), ops.get("key_lengths")
-    dq = torch.empty((B, Sq, H, D), dtype=q.dtype, device=device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=device)
+    dq, dk, dv = q.new_empty((B, Sq, H, D)), k.new_empty(k.shape), k.new_empty(k.shape)
     desc = _attention_desc(q, k, v, causal, scale)
     lib = _lib.lib()
     need = lib.mia_attention_backward_workspace_bytes(ctypes.byref(desc))
-    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _call(lib.mia_attention_backward, device, ctypes.byref(desc), dout.data_ptr(), _strides(dout), q.data_ptr(),
           k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(out), lse.data_ptr(), _ptr(lengths), dq.data_ptr(),
           dk.data_ptr(), dv.data_ptr(), _ptr(ws), need)

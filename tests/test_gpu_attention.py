@@ -173,7 +173,7 @@ def test_views_and_alignment(gpu, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
 def test_many_workgroups(gpu, t, dim):
     """Enough rows for the wider workgroups, forward and backward."""
     t = TYPES[t]
@@ -227,3 +227,37 @@ def test_two_calls_give_the_same_bits(gpu):
     first = attention_backward(out, q, k, k, out, lse)
     for _ in range(3):
         assert all(torch.equal(a, c) for a, c in zip(first, attention_backward(out, q, k, k, out, lse)))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_many_items_and_split_keys_with_lengths(gpu, t):
+    t = TYPES[t]
+    lengths = [(17 * i) % 41 for i in range(70)]        # more items than a wave has lanes, lengths 0 ... 40
+    q, k, v = make((70, 33, 1, 64), t, 25), make((70, 40, 1, 64), t, 26), make((70, 40, 1, 64), t, 27)
+    check(q, k, v, False, lengths)
+    q, k, v = make((3, 1, 4, 64), t, 28), make((3, 1500, 2, 64), t, 29), make((3, 1500, 2, 64), t, 30)
+    for lengths in ([0, 700, 1500], [1, 256, 257]):
+        for b, n in enumerate(lengths):
+            k[b, n:], v[b, n:] = float("nan"), float("nan")
+        check(q, k, v, False, lengths)
+        check(q, k, v, True, lengths)
+        k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+
+
+def test_a_cache_beyond_four_gigabytes(gpu):
+    """Keys whose offsets pass 32 bits, in elements as well as bytes: the last head's keys and values
+    against a compact copy of them, bit for bit."""
+    Sk, Hk = 300_000, 64
+    kv = torch.zeros((2, 1, Sk, Hk, 128), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(31)
+    kv[:, :, :, 63:] = torch.randn((2, 1, Sk, 1, 128), generator=g, device="cuda").to(torch.bfloat16)
+    k, v = kv[0, :, :, 63:], kv[1, :, :, 63:]
+    q = torch.randn((1, 2, 1, 128), generator=g, device="cuda").to(torch.bfloat16)
+    for n in (Sk, Sk - 7):
+        out, lse = attention(q, k, v, key_lengths=[n], return_lse=True)
+        kc, vc = k.contiguous(), v.contiguous()
+        want, wlse = attention(q, kc, vc, key_lengths=[n], return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, wlse)
+        got = attention_backward(out, q, k, v, out, lse, key_lengths=[n])
+        ref = attention_backward(out, q, kc, vc, out, lse, key_lengths=[n])
+        assert all(torch.equal(a, c) for a, c in zip(got, ref))

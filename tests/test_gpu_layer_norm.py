@@ -157,3 +157,20 @@ def test_two_calls_give_the_same_bits(gpu):
     first = layer_norm_backward(dy, x, mean, rstd, w)
     for _ in range(3):
         assert all(torch.equal(a, c) for a, c in zip(first, layer_norm_backward(dy, x, mean, rstd, w)))
+
+
+def test_rows_beyond_four_gigabytes(gpu):
+    m, n = 2_200_000, 1024
+    x = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+    x[-5:] = make((5, n), torch.bfloat16, 20)
+    w = make((n,), torch.bfloat16, 21, 1.0, 0.1)
+    y, mean, rstd = layer_norm(x, w, return_stats=True)
+    want = layer_norm(x[-5:].clone(), w, return_stats=True)
+    assert all(torch.equal(a[-5:], c) for a, c in zip((y, mean, rstd), want)) and (y[:-5] == 0).all()
+    dx, dw, db = layer_norm_backward(y, x, mean, rstd, w)
+    ref = layer_norm_backward(y[-5:].clone(), x[-5:].clone(), mean[-5:], rstd[-5:], w)
+    assert torch.equal(dx[-5:], ref[0]) and (dx[:-5] == 0).all()
+    # five rows that are not zero, added in another order: 4 * 2^-24 of their magnitudes
+    h = (f64(x[-5:]) - f64(mean[-5:])[:, None]) * f64(rstd[-5:])[:, None]
+    assert (np.abs(f64(dw) - f64(ref[1])) <= 8 * 2.0 ** -24 * np.abs(f64(y[-5:]) * h).sum(0) + 1e-30).all()
+    assert (np.abs(f64(db) - f64(ref[2])) <= 8 * 2.0 ** -24 * np.abs(f64(y[-5:])).sum(0) + 1e-30).all()

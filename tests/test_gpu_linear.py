@@ -187,3 +187,24 @@ def test_two_calls_give_the_same_bits(gpu):
     first = linear_backward(dy, x, w, activation="gelu", preactivation=z)
     for _ in range(3):
         assert all(torch.equal(a, c) for a, c in zip(first, linear_backward(dy, x, w, activation="gelu", preactivation=z)))
+
+
+def test_rows_beyond_four_gigabytes(gpu):
+    """Row offsets that pass 32 bits: the last rows against a call on a copy of them, bit for bit."""
+    m, k, n = 2_200_000, 1024, 64
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    x[-300:] = make((300, k), torch.bfloat16, 34)
+    w = make((n, k), torch.bfloat16, 35, k ** -0.5)
+    y = linear(x, w)
+    want, _ = o.linear(f64(x[-300:]), f64(w))
+    acc = (k + 4) * 2.0 ** -23 * (np.abs(f64(x[-300:])) @ np.abs(f64(w)).T)
+    assert (np.abs(f64(y[-300:]) - want) <= u(torch.bfloat16) * np.abs(want) * (1 + 1e-6) + acc).all()
+    assert (y[:-300] == 0).all()
+    dx, dw, db = linear_backward(y, x, w)
+    assert (dx[:-300] == 0).all() and torch.isfinite(dx[-300:].float()).all() and dx[-1].abs().sum() > 0
+    ex, ew, eb = o.linear_backward(f64(y[-300:]), f64(x[-300:]), f64(w))
+    dy = np.abs(f64(y[-300:]))
+    tol = u(torch.bfloat16) * np.abs(ew) * (1 + 1e-6) + 304 * 2.0 ** -23 * (dy.T @ np.abs(f64(x[-300:]))) + 1e-30
+    assert (np.abs(f64(dw) - ew) <= tol).all()
+    tol = u(torch.bfloat16) * np.abs(ex) * (1 + 1e-6) + 68 * 2.0 ** -23 * (dy @ np.abs(f64(w))) + 1e-30
+    assert (np.abs(f64(dx[-300:]) - ex) <= tol).all()
