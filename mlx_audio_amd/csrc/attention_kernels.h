@@ -277,7 +277,10 @@ __device__ __forceinline__ float column_sum(float v) {
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 }  // namespace att
 
-// Forward.  OT: blocks of 16 queries per wave.
+// Forward.  OT: blocks of 16 queries per wave.  bfloat16, 8 x 1500, 20 heads of 64: 139 us (663 TFLOP/s), bound by the
+// vector ALUs: 209 instructions beside 32 matrix ones for 64 keys x 32 queries.  Four waves per SIMD (128 registers)
+// instead of three: 157 -> 140.  4 x 2048, 16 heads of 128: 148 us (927).  One query on 1500 keys, 16 items, 20 heads:
+// 26 us with the join, HBM.
 template <class T, int DP, int OT, bool DMA>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_fwd_kernel(att::Args p) {
   using namespace att;
@@ -650,7 +653,8 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   }
 }
 
-// dk and dv: own rows are keys, q and dout stream, over all heads that share the key head.
+// dk and dv: own rows are keys, q and dout stream, over all heads that share the key head.  With dq, bfloat16,
+// 8 x 1500, 20 heads of 64: 410 us.  Two waves per SIMD: for three the registers spill (438 -> 552 us).
 template <class T, int DP, int OT, bool DMA>
 __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_kernel(att::Args p) {
   using namespace att;

@@ -7,7 +7,7 @@
 //   dW        A = x  (k, n)  n contiguous      B = dz (k, m)  m contiguous
 //
 // (k is what is summed over, n the result's contiguous index.)  An operand whose k is contiguous
-// lies in LDS as rows of 64 bytes of k and a lane's 16-byte fragment is one ds_read_b128; the other
+// lies in LDS as rows of 128 bytes of k and a lane's 16-byte fragment is one ds_read_b128; the other
 // kind lies as rows of n (or m) and fragments are taken down the columns: ds_read_b64_tr_b16 for
 // two-byte types, four ds_read_b32 for float.  Nothing is transposed in memory.
 #pragma once
@@ -40,7 +40,8 @@ struct Gemm {
   Epilogue e;
 };
 
-// 0.5 erfc(-x / sqrt 2) from erfc(z) = t (a1 + t (a2 + ... a5 t)) exp(-z^2), t = 1 / (1 + p z):
+// 0.5 erfc(-x / sqrt 2) from erfc(z) = t (a1 + t (a2 + ... a5 t)) exp(-z^2), t = 1 / (1 + p z)
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26):
 // absolute error 1.5e-7 and no cancellation in the negative tail; `e` receives exp(-x^2 / 2).
 __device__ __forceinline__ float normal_cdf_fast(float x, float& e) {
   const float z = __builtin_fabsf(x) * 0.70710678118654752440f;
@@ -481,7 +482,8 @@ struct Part {
 }  // namespace lin
 
 // Four waves, one tile per workgroup; several workgroups share a compute unit and fill each other's
-// gaps.  DMA: every 16-byte piece of both operands is aligned (bases, row strides) and lies either
+// gaps (dW of 24000 x 1280 -> 5120, bfloat16: 334 us here, 352 with the 256 tile in two parts; float32,
+// 6000 x 5120 -> 1280: 600 us, 131 TFLOP/s).  DMA: every 16-byte piece of both operands is aligned (bases, row strides) and lies either
 // wholly inside its operand or wholly outside; otherwise pieces go through registers, element by
 // element at the edges.
 template <class TL, class T, bool AKC, bool BKC, bool DMA>
@@ -567,6 +569,9 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
 // buffer of stage g as soon as all waves have read that, one stage before its use.  So at the end of
 // a tile the results are stored while the next tile's first stages arrive; a wave waits for its loads,
 // never for the stores behind them (loads and stores are counted in order: "all but the newest STORES").
+// Measured, bfloat16: 8192^3 802 us (1 372 TFLOP/s); 24000 x 1280 -> 5120 351 us (897; with GELU and the
+// preactivation 388), 24000 x 5120 -> 1280 259 (1 214).  A stage takes 1.57 us, of which the matrix instructions
+// need 0.85 at 2.4 GHz; reading fragments and multiplying share the rest.  Short k is bound by the tile's end.
 template <class TL, class T, bool AKC, bool BKC>
 __global__ __launch_bounds__(TL::WG, 1) void lin_gemm8_kernel(lin::Gemm p) {
   using namespace lin;
@@ -665,6 +670,7 @@ __global__ __launch_bounds__(256) void lin_join_kernel(lin::Gemm p) {
 // Few rows of x (MT groups of 16): a stream through the weights.  A workgroup owns 16 columns of
 // the result, its waves take 64-byte steps of k in turn and their sums meet in LDS.  Fragments come
 // straight from memory: 16 bytes a lane, 64 bytes of each of 16 weight rows per load.
+// 8 x 1280 -> 5120, bfloat16, GELU: 8 us for 13 MB of weights; a call takes 12, bound by the host.
 template <class T, int MT, int NW>
 __global__ __launch_bounds__(64 * NW) void lin_few_kernel(lin::Gemm p) {
   using namespace lin;
@@ -726,7 +732,7 @@ __global__ __launch_bounds__(64 * NW) void lin_few_kernel(lin::Gemm p) {
 
 // dz = dy act'(z), rounded to the operands' type for the two products that read it, and the column
 // sums of the unrounded values: workgroup (x, y) takes rows y, y + gridDim.y ... of 64 pieces of 16
-// bytes, four rows at a time (one per wave).  z null: no activation, sums only (dz null too).
+// bytes, four rows at a time (one per wave).  24000 x 5120, bfloat16: 150 us, 4.9 TB/s.  z null: no activation, sums only (dz null too).
 template <class T>
 __global__ __launch_bounds__(256) void lin_dz_kernel(const T* __restrict__ dy, long long dy_stride,
                                                      const T* __restrict__ z, long long z_stride, int act, int m,
