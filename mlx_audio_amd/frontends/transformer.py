@@ -25,6 +25,7 @@ from .. import _lib
 from .._runtime import require_gpu
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_INTEGERS = (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64)
 _ACTIVATIONS = {None: _lib.ACT_NONE, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH, "relu": _lib.ACT_RELU}
 
 
@@ -293,12 +294,12 @@ def _check_lengths(lengths, batch: int, keys: int):
     """key_lengths as an int32 tensor (host or device); host values are checked."""
     if not isinstance(lengths, torch.Tensor):
         lengths = torch.as_tensor(np.asarray(lengths))
-    if lengths.shape != (batch,) or lengths.dtype.is_floating_point or lengths.dtype in (torch.bool, torch.complex64):
+    if lengths.shape != (batch,) or lengths.dtype not in _INTEGERS:
         raise ValueError(f"key_lengths must be {batch} integers, got {lengths.dtype} {tuple(lengths.shape)}")
     if not lengths.is_cuda and batch and not 0 <= int(lengths.min()) <= int(lengths.max()) <= keys:
         raise ValueError(f"key_lengths must lie in 0 .. {keys}")
     if lengths.dtype != torch.int32:
-        lengths = lengths.clamp(0, keys).to(torch.int32)
+        lengths = lengths.to(torch.int64).clamp(0, keys).to(torch.int32)  # (keys need not fit the given type)
     return lengths.contiguous()
 
 
