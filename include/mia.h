@@ -624,6 +624,8 @@ int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_
  * contiguous [batch, queries, heads, dim] of q's type; lse: float32 (batch, heads, queries), the
  * logarithm of the sum of exponentials, or NULL (the backward pass needs it).  A value that is not
  * finite in a key or value row that SOME query of a causal call sees may reach other queries.
+ * A call may have fewer than 2^24 workgroups of 64 or 128 rows (of each batch item and head, parts
+ * of a split included): MIA_ERR_UNSUPPORTED beyond, before anything is enqueued.
  * workspace: mia_attention_workspace_bytes bytes, 16-byte aligned (0 unless the keys are split). */
 typedef struct mia_attention_desc {
   int dtype;

@@ -233,8 +233,14 @@ __device__ __forceinline__ void store_own(T* row, int dim, int lane, const f4 (&
 // Workgroups go to the eight XCDs in turn; all of a pair go to one XCD, whose L2 then holds its keys
 // and values, and the pairs go round the XCDs, so that items of different lengths spread evenly.
 // With few pairs (less than 64) that would leave XCDs without work: in order then.  False: none.
-static inline unsigned order_grid(long long pairs, long long per) {
-  return (unsigned)(pairs < 64 ? pairs * per : (pairs + 7) / 8 * 8 * per);
+static inline long long order_grid(long long pairs, long long per) {
+  return pairs < 64 ? pairs * per : (pairs + 7) / 8 * 8 * per;
+}
+// A launch counts its threads in 32 bits; nothing is enqueued that does not fit.
+static inline int check_grid(long long grid) {
+  if (grid < (1LL << 24)) return MIA_OK;
+  set_error("too many rows for one call (%lld workgroups)", grid);
+  return MIA_ERR_UNSUPPORTED;
 }
 __device__ __forceinline__ bool order(unsigned pairs, unsigned per, unsigned& pair, unsigned& index) {
   if (pairs < 64) {
@@ -905,7 +911,7 @@ static bool pieces_ok(const View& v, size_t es) {
   return aligned16(v.p) && v.b % n == 0 && v.s % n == 0 && v.h % n == 0 && v.s * (long long)es < (1LL << 25);
 }
 #define MIA_ATT_ONE(kernel, dp, ot, grid) \
-  hipLaunchKernelGGL((kernel<T, dp, ot, decltype(dma)::value>), dim3(grid), dim3(256), 0, s, a)
+  hipLaunchKernelGGL((kernel<T, dp, ot, decltype(dma)::value>), dim3((unsigned)(grid)), dim3(256), 0, s, a)
 #define MIA_ATT_LAUNCH(kernel, ot, grid)                 \
   do {                                                   \
     if (a.dim <= 32) MIA_ATT_ONE(kernel, 32, ot, grid);  \
@@ -924,7 +930,9 @@ template <class T>
 int Ops<T>::forward(Args a, hipStream_t s) {
   const Plan pl = plan_forward(a.batch, a.sq, a.sk, a.heads, a.kv_heads);
   a.pack = pl.pack, a.own_tiles = pl.own_tiles, a.splits = pl.splits, a.keys_per_split = pl.keys_per_split;
-  const unsigned grid = order_grid((long long)a.batch * (a.heads / a.pack), (long long)a.own_tiles * a.splits);
+  const long long grid = order_grid((long long)a.batch * (a.heads / a.pack), (long long)a.own_tiles * a.splits);
+  const int rc = check_grid(grid);
+  if (rc != MIA_OK) return rc;
   const bool dma = a.dim % (16 / (int)sizeof(T)) == 0 && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T));
   with_dma(dma, [&](auto dma) { 
     if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_fwd_kernel, 2, grid);
@@ -940,6 +948,12 @@ template <class T>
 int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStream_t s) {
   const long long rows = (long long)a.batch * a.heads * a.sq;
   const bool whole = a.dim % (16 / (int)sizeof(T)) == 0;
+  const GradPlan of_dq = plan_dq(a.batch, a.sq, a.sk, a.heads, sizeof(T));
+  const GradPlan of_dkv = plan_dkv(a.batch, a.sq, a.sk, a.heads, a.kv_heads, a.dim, sizeof(T));
+  const long long dq_grid = order_grid((long long)a.batch * a.heads, (long long)of_dq.own_tiles * of_dq.splits);
+  const long long dkv_grid = order_grid((long long)a.batch * a.kv_heads, (long long)of_dkv.own_tiles * of_dkv.splits);
+  const int rc = check_grid(dq_grid > dkv_grid ? dq_grid : dkv_grid);
+  if (rc != MIA_OK) return rc;
   a.stats = stats, a.pack = 1;
   a.partial = stats + align256((size_t)2 * rows * sizeof(float)) / sizeof(float);
   auto add = [&](long long total, long long n, void* out0, void* out1) {
@@ -948,31 +962,27 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
                        total, a.splits, n, static_cast<T*>(out0), static_cast<T*>(out1));
   };
   if (rows) {
-    const GradPlan pl = plan_dq(a.batch, a.sq, a.sk, a.heads, sizeof(T));
-    a.own_tiles = pl.own_tiles, a.splits = pl.splits;
+    a.own_tiles = of_dq.own_tiles, a.splits = of_dq.splits;
     a.o0 = dq, a.o1 = nullptr;
-    const unsigned grid = order_grid((long long)a.batch * a.heads, (long long)a.own_tiles * a.splits);
     with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)), [&](auto dma) {
-      if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_dq_kernel, 2, grid);
-      else MIA_ATT_LAUNCH(att_dq_kernel, 1, grid);
+      if (of_dq.own_blocks == 2) MIA_ATT_LAUNCH(att_dq_kernel, 2, dq_grid);
+      else MIA_ATT_LAUNCH(att_dq_kernel, 1, dq_grid);
     });
     if (a.splits > 1) add(rows * a.dim, rows * a.dim, dq, nullptr);
   }
   if (a.sk) {
-    const GradPlan pl = plan_dkv(a.batch, a.sq, a.sk, a.heads, a.kv_heads, a.dim, sizeof(T));
-    a.own_tiles = pl.own_tiles, a.splits = pl.splits;
+    a.own_tiles = of_dkv.own_tiles, a.splits = of_dkv.splits;
     a.o0 = dk, a.o1 = dv;
-    const unsigned grid = order_grid((long long)a.batch * a.kv_heads, (long long)a.own_tiles * a.splits);
     with_dma(whole && pieces_ok(a.q, sizeof(T)) && pieces_ok(a.dout, sizeof(T)), [&](auto dma) {
-      if (pl.own_blocks == 2) {
+      if (of_dkv.own_blocks == 2) {
         if constexpr (sizeof(T) == 2) {
-          if (a.dim <= 32) MIA_ATT_ONE(att_dkv_kernel, 32, 2, grid);
-          else MIA_ATT_ONE(att_dkv_kernel, 64, 2, grid);
+          if (a.dim <= 32) MIA_ATT_ONE(att_dkv_kernel, 32, 2, dkv_grid);
+          else MIA_ATT_ONE(att_dkv_kernel, 64, 2, dkv_grid);
         } else {
-          MIA_ATT_ONE(att_dkv_kernel, 32, 2, grid);
+          MIA_ATT_ONE(att_dkv_kernel, 32, 2, dkv_grid);
         }
       } else {
-        MIA_ATT_LAUNCH(att_dkv_kernel, 1, grid);
+        MIA_ATT_LAUNCH(att_dkv_kernel, 1, dkv_grid);
       }
     });
     if (a.splits > 1) {

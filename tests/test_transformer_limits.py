@@ -23,3 +23,22 @@ def test_key_lengths_that_are_no_integers_are_refused(dtype):
     q = torch.empty(2, 3, 4, 16)
     with pytest.raises(ValueError, match="key_lengths"):
         f.attention(q, q, q, key_lengths=torch.zeros(2).to(dtype))
+
+
+def attention_desc(**kw):
+    d = dict(dtype=0, batch=1, queries=2, keys=3, heads=4, kv_heads=2, dim=16, causal=0, scale=0.25)
+    d.update(kw)
+    s = (ctypes.c_int64 * 3)(1, 1, 1)
+    return ctypes.byref(_lib.AttentionDesc(**d, stride_q=s, stride_k=s, stride_v=s))
+
+
+def test_attention_refuses_more_workgroups_than_one_launch_holds():
+    """A launch counts its threads in 32 bits: 2^24 workgroups of 256."""
+    lib = _lib.lib()
+    s = (ctypes.c_int64 * 3)(1, 1, 1)
+    many = attention_desc(batch=1 << 24, queries=1)
+    assert lib.mia_attention(many, P, P, P, None, P, None, None, 0, None) == _lib.MIA_ERR_UNSUPPORTED
+    assert lib.mia_attention_backward(many, P, s, P, P, P, P, s, P, None, P, P, P, P, 1 << 40, None) == _lib.MIA_ERR_UNSUPPORTED
+    # dk / dv alone is too large: refused before dq is enqueued
+    keys = attention_desc(batch=1 << 20, queries=1, keys=4096, heads=1, kv_heads=1)
+    assert lib.mia_attention_backward(keys, P, s, P, P, P, P, s, P, None, P, P, P, P, 1 << 62, None) == _lib.MIA_ERR_UNSUPPORTED
