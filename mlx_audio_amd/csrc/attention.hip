@@ -12,7 +12,8 @@ static int check(const mia_attention_desc* d) {
   MIA_REQUIRE(d->heads >= 1 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0,
               "heads must be a multiple of kv_heads (got %d, %d)", d->heads, d->kv_heads);
   MIA_REQUIRE(d->dim >= 1, "dim must be positive (got %d)", d->dim);
-  MIA_REQUIRE(d->scale > 0.0f && d->scale < __builtin_huge_valf(), "scale must be positive and finite");
+  // (exponents are taken to base 2: scale / ln 2 has to be finite as well)
+  MIA_REQUIRE(d->scale > 0.0f && d->scale * kLog2e < __builtin_huge_valf(), "scale must be positive and below 2.3e38");
   for (const int64_t* s = d->stride_q; s < d->stride_q + 3; ++s) MIA_REQUIRE(*s >= 0, "strides must not be negative");
   for (const int64_t* s = d->stride_k; s < d->stride_k + 3; ++s) MIA_REQUIRE(*s >= 0, "strides must not be negative");
   for (const int64_t* s = d->stride_v; s < d->stride_v + 3; ++s) MIA_REQUIRE(*s >= 0, "strides must not be negative");

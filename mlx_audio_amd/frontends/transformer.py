@@ -285,7 +285,7 @@ def _check_attention(q, k, v, scale) -> float:
     if D > 128:
         raise NotImplementedError(f"head dimensions beyond 128 are not supported (got {D})")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
+    if not 0.0 < scale < 2.3e38:  # (what float32 exponents to base 2 can be taken with)
         raise ValueError(f"scale must be positive and finite (got {scale})")
     return scale
 

@@ -42,3 +42,10 @@ def test_attention_refuses_more_workgroups_than_one_launch_holds():
     # dk / dv alone is too large: refused before dq is enqueued
     keys = attention_desc(batch=1 << 20, queries=1, keys=4096, heads=1, kv_heads=1)
     assert lib.mia_attention_backward(keys, P, s, P, P, P, P, s, P, None, P, P, P, P, 1 << 62, None) == _lib.MIA_ERR_UNSUPPORTED
+
+
+def test_attention_refuses_a_scale_that_overflows():
+    """Exponents are taken to base 2: scale / ln 2 has to be finite as well."""
+    lib = _lib.lib()
+    assert lib.mia_attention(attention_desc(scale=3e38), P, P, P, None, P, None, None, 0, None) == _lib.MIA_ERR_INVALID
+    assert lib.mia_attention(attention_desc(scale=3e38, batch=0), P, P, P, None, P, None, None, 0, None) == _lib.MIA_ERR_INVALID
