@@ -32,14 +32,15 @@ __global__ __launch_bounds__(1024) void lin_bias_join_kernel(const float* __rest
 
 namespace lin {
 constexpr long long kMaxSize = (1LL << 30) - 4096;  // positions along k are counted in 32 bits
+constexpr long long kMaxWidth = 1LL << 26;          // and so are a launch's threads (up to 32 a column)
 constexpr int kBiasGroups = 256;
 // at least sixteen rows each
 static int bias_groups(long long m) { return (int)((m + 15) / 16 < kBiasGroups ? (m + 15) / 16 : kBiasGroups); }
 
 static int check(long long m, long long n, long long k, int dtype) {
   MIA_REQUIRE(m >= 0 && n >= 1 && k >= 1, "rows must be >= 0 and both widths >= 1 (got %lld rows, %lld -> %lld)", m, k, n);
-  if (m > kMaxSize || n > kMaxSize || k > kMaxSize) {
-    set_error("sizes beyond 2^30 - 4096 are not supported");
+  if (m > kMaxSize || n > kMaxWidth || k > kMaxWidth) {
+    set_error("more than 2^30 - 4096 rows or widths beyond 2^26 are not supported");
     return MIA_ERR_UNSUPPORTED;
   }
   MIA_REQUIRE(dtype_ok(dtype), "unknown dtype %d", dtype);

@@ -807,11 +807,12 @@ static Choice choose(long long n, long long m, long long k, size_t es, bool dma,
   static const Kind kinds[3] = {{256, 1, 1.6, 7.2, 6.0}, {128, 2, 0.88, 3.6, 4.0}, {64, 4, 0.83, 1.8, 3.0}};
   const int kstep = (int)(128 / es);
   const long long steps = (k + kstep - 1) / kstep;
-  Choice best{64, 1, 0};
+  Choice best{128, 1, 0};  // (too large for any: refused when launched)
   double least = 0.0;
   for (const Kind& kd : kinds) {
     if (kd.tile == 256 && !dma) continue;
     const long long tiles = tiles_of(n, m, kd.tile);
+    if (kd.tile != 256 && tiles * 32 >= (1LL << 24)) continue;  // more threads than a launch counts
     for (int splits = 1; splits <= 32 && (splits == 1 || steps / splits >= 4); ++splits) {
       const long long groups = tiles * splits, per_cu = (groups + kCus - 1) / kCus;
       const double load = per_cu < kd.per_cu ? (double)per_cu / kd.per_cu : 1.0;  // a stage is faster alone
@@ -841,7 +842,8 @@ static int launch(Gemm g, hipStream_t s) {
   g.n_tiles = (g.n + TL::BN - 1) / TL::BN;
   g.m_tiles = (g.m + TL::BM - 1) / TL::BM;
   const long long blocks = (long long)g.n_tiles * g.m_tiles * g.splits;
-  if (blocks >= (1LL << 31)) {
+  // a launch counts its threads in 32 bits (the kernel of eight waves walks its tiles: 31 bits of them)
+  if (blocks >= (TL::NW == 8 ? 1LL << 31 : (1LL << 32) / TL::WG)) {
     set_error("product too large for one launch");
     return MIA_ERR_UNSUPPORTED;
   }

@@ -49,3 +49,18 @@ def test_attention_refuses_a_scale_that_overflows():
     lib = _lib.lib()
     assert lib.mia_attention(attention_desc(scale=3e38), P, P, P, None, P, None, None, 0, None) == _lib.MIA_ERR_INVALID
     assert lib.mia_attention(attention_desc(scale=3e38, batch=0), P, P, P, None, P, None, None, 0, None) == _lib.MIA_ERR_INVALID
+
+
+def test_linear_refuses_more_workgroups_than_one_launch_holds():
+    lib = _lib.lib()
+
+    def linear(rows, k, n):
+        return lib.mia_linear(P, k, P, k, None, 0, None, 0, 0, rows, k, n, 0, P, None, P, 1 << 62, None)
+
+    wide = (1 << 26) + 1
+    for rows, k, n in ((1, 8, wide), (1, wide, 8), (100, 8, wide)):
+        assert linear(rows, k, n) == _lib.MIA_ERR_UNSUPPORTED
+    # rows of seven elements go through registers: no kernel there that walks tiles
+    assert linear((1 << 30) - 4096, 7, 1000) == _lib.MIA_ERR_UNSUPPORTED
+    assert lib.mia_linear_backward(P, wide, P, 8, P, 8, None, 0, 0, 1, 8, wide, 0, P, P, P, P, 1 << 62,
+                                   None) == _lib.MIA_ERR_UNSUPPORTED
