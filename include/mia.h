@@ -579,7 +579,7 @@ int mia_whisper_stem(const float* mel, int64_t clips, int64_t frames, int n_mels
 #define MIA_BF16 2
 
 /* y[r] = (x[r] - mean) * rstd * weight + bias over rows of dim elements, rstd = 1 / sqrt(variance
- * + eps).  weight, bias: device (dim), float32 or x's type (param_dtype, both alike), either may
+ * + eps); dim up to 2^25, rows below 2^31 (2^24 where dim > 8192).  weight, bias: device (dim), float32 or x's type (param_dtype, both alike), either may
  * be NULL; y: (rows, dim) contiguous; mean, rstd: device float32 (rows), or both NULL. */
 int mia_layer_norm(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int dtype, const void* weight,
                    const void* bias, int param_dtype, float eps, void* y, float* mean, float* rstd, void* stream);

@@ -365,7 +365,10 @@ static void launch_bwd(const Args& a, int groups, hipStream_t s) {
 
 static int check(long long rows, long long dim, int dtype, const void* w, const void* b, int param_dtype) {
   MIA_REQUIRE(rows >= 0 && rows < (1LL << 31), "rows must be in 0 .. 2^31 - 1 (got %lld)", rows);
-  MIA_REQUIRE(dim >= 1 && dim < (1LL << 28), "dim must be in 1 .. 2^28 - 1 (got %lld)", dim);
+  // (a launch counts its threads in 32 bits: 64 a column in the join, 256 a long row)
+  MIA_REQUIRE(dim >= 1 && dim <= (1LL << 25), "dim must be in 1 .. 2^25 (got %lld)", dim);
+  MIA_REQUIRE(dim <= kRegisterDim || rows < (1LL << 24), "rows of more than %d elements: at most 2^24 - 1 (got %lld)",
+              kRegisterDim, rows);
   MIA_REQUIRE(dtype_ok(dtype), "unknown dtype %d", dtype);
   MIA_REQUIRE((!w && !b) || param_dtype == dtype || param_dtype == MIA_F32,
               "parameters must be float32 or of the input's type");

@@ -64,3 +64,18 @@ def test_linear_refuses_more_workgroups_than_one_launch_holds():
     assert linear((1 << 30) - 4096, 7, 1000) == _lib.MIA_ERR_UNSUPPORTED
     assert lib.mia_linear_backward(P, wide, P, 8, P, 8, None, 0, 0, 1, 8, wide, 0, P, P, P, P, 1 << 62,
                                    None) == _lib.MIA_ERR_UNSUPPORTED
+
+
+def test_layer_norm_refuses_more_workgroups_than_one_launch_holds():
+    lib = _lib.lib()
+    wide = (1 << 25) + 1
+
+    def forward(rows, dim):
+        return lib.mia_layer_norm(P, rows, dim, dim, 0, None, None, 0, 1e-5, P, None, None, None)
+
+    def backward(rows, dim):
+        return lib.mia_layer_norm_backward(P, dim, P, dim, P, P, rows, dim, 0, P, 0, P, P, P, P, 1 << 62, None)
+
+    for rows, dim in ((1, wide), (1 << 24, 8193)):
+        assert forward(rows, dim) == _lib.MIA_ERR_INVALID
+        assert backward(rows, dim) == _lib.MIA_ERR_INVALID
