@@ -584,7 +584,7 @@ int mia_whisper_stem(const float* mel, int64_t clips, int64_t frames, int n_mels
 int mia_layer_norm(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int dtype, const void* weight,
                    const void* bias, int param_dtype, float eps, void* y, float* mean, float* rstd, void* stream);
 /* The gradients, from the statistics the forward call wrote: dx (rows, dim) contiguous of x's type;
- * dweight, dbias: float32 (dim), or both NULL (then no workspace is needed). */
+ * dweight, dbias: float32 (dim), or both NULL (then no workspace is needed); workspace: 16-byte aligned. */
 size_t mia_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
 int mia_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
                             const float* rstd, int64_t rows, int64_t dim, int dtype, const void* weight,

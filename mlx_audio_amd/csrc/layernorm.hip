@@ -417,8 +417,9 @@ int mia_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
   MIA_REQUIRE(rows == 0 || (dy && x && mean && rstd && dx), "null argument");
   MIA_REQUIRE(dy_stride >= 0 && x_stride >= 0, "rows must not run backwards");
   MIA_REQUIRE(!dweight || rows == 0 ||
-                  (workspace && workspace_bytes >= mia_layer_norm_backward_workspace_bytes(rows, dim)),
-              "workspace too small");
+                  (workspace && workspace_bytes >= mia_layer_norm_backward_workspace_bytes(rows, dim) &&
+                   nn::aligned16(workspace)),
+              "workspace too small or not aligned to 16 bytes");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int groups = rows ? ln::groups_of(rows, dim) : 0;
   if (rows) {

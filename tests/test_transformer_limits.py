@@ -79,3 +79,9 @@ def test_layer_norm_refuses_more_workgroups_than_one_launch_holds():
     for rows, dim in ((1, wide), (1 << 24, 8193)):
         assert forward(rows, dim) == _lib.MIA_ERR_INVALID
         assert backward(rows, dim) == _lib.MIA_ERR_INVALID
+
+
+def test_layer_norm_backward_refuses_a_workspace_that_is_not_aligned():
+    lib = _lib.lib()
+    odd = ctypes.c_void_p(257)
+    assert lib.mia_layer_norm_backward(P, 8, P, 8, P, P, 2, 8, 0, P, 0, P, P, P, odd, 1 << 20, None) == _lib.MIA_ERR_INVALID
