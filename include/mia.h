@@ -597,7 +597,7 @@ int mia_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
  * and preactivation: (rows, out) contiguous; neither may overlap an input.  GELU is the erf form,
  * GELU_TANH its tanh approximation.  workspace: mia_linear_workspace_bytes bytes of device memory,
  * 16-byte aligned (often 0).  Up to 2^30 - 4096 rows and widths up to 2^26; operands whose rows are
- * not aligned to 16 bytes: results up to about 2^33 (MIA_ERR_UNSUPPORTED beyond). */
+ * not aligned to 16 bytes: fewer than 2^24 tiles of 128 x 128 results (MIA_ERR_UNSUPPORTED beyond). */
 #define MIA_ACT_NONE 0
 #define MIA_ACT_GELU 1
 #define MIA_ACT_GELU_TANH 2

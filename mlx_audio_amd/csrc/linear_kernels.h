@@ -812,9 +812,9 @@ static Choice choose(long long n, long long m, long long k, size_t es, bool dma,
   for (const Kind& kd : kinds) {
     if (kd.tile == 256 && !dma) continue;
     const long long tiles = tiles_of(n, m, kd.tile);
-    if (kd.tile != 256 && tiles * 32 >= (1LL << 24)) continue;  // more threads than a launch counts
     for (int splits = 1; splits <= 32 && (splits == 1 || steps / splits >= 4); ++splits) {
       const long long groups = tiles * splits, per_cu = (groups + kCus - 1) / kCus;
+      if (kd.tile != 256 && groups >= (1LL << 24)) break;  // more threads than a launch counts
       const double load = per_cu < kd.per_cu ? (double)per_cu / kd.per_cu : 1.0;  // a stage is faster alone
       double stage = (es == 4 ? kd.stage4 : kd.stage2) * (0.45 + 0.55 * load);
       if (!dma) stage *= kd.tile == 64 ? 1.6 : columns ? 3.4 : 1.9;  // pieces through registers

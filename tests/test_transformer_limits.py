@@ -85,3 +85,9 @@ def test_layer_norm_backward_refuses_a_workspace_that_is_not_aligned():
     lib = _lib.lib()
     odd = ctypes.c_void_p(257)
     assert lib.mia_layer_norm_backward(P, 8, P, 8, P, P, 2, 8, 0, P, 0, P, P, P, odd, 1 << 20, None) == _lib.MIA_ERR_INVALID
+
+
+def test_linear_serves_a_long_result_that_goes_through_registers():
+    """2^23 tiles of one launch: planned, and refused here only for what else is wrong (no weight)."""
+    lib = _lib.lib()
+    assert lib.mia_linear_workspace_bytes((1 << 30) - 4096, 7, 1, 0) == 0  # one part of k
