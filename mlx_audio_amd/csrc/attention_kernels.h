@@ -287,7 +287,12 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // vector ALUs: 209 instructions beside 32 matrix ones for 64 keys x 32 queries.  Four waves per SIMD (128 registers)
 // instead of three: 157 -> 140.  4 x 2048, 16 heads of 128: 148 us (927).  One query on 1500 keys, 16 items, 20 heads:
 // 26 us with the join, HBM.
-template <class T, int DP, int OT, bool DMA>
+// BOTH: what the rounding of p to a two-byte type takes away goes through a second product, and the error falls from
+// 1.39 to 1.00 of a result rounded once.  For calls whose rows (up to 64 of a pair) fit one workgroup, as a decoding
+// step's do: memory sets their time and the matrix units are idle (16 x 1 on
+// 1500 keys, 20 heads of 64: 26.8 -> 26.9 us; 4 x 1 on 4096, 32 heads over 4 of 128: 27.7 -> 28.4; 1 x 1: 12.0 -> 12.4).  Not with more rows, where it costs
+// 7 - 20 % (1 x 1500, 20 heads of 64: 40 -> 46 us).
+template <class T, int DP, int OT, bool DMA, bool BOTH>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_fwd_kernel(att::Args p) {
   using namespace att;
   using S = Shape<T, DP>;
@@ -430,19 +435,29 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
     }
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
-      u4 pf[OT];
+      u4 pf[OT], rest[OT];
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
         f4 blocks[S::RB];
 #pragma unroll
         for (int r = 0; r < S::RB; ++r) blocks[r] = s[st * S::RB + r][o];
         pf[o] = to_operand<T>(blocks);
+        if constexpr (BOTH) {
+#pragma unroll
+          for (int r = 0; r < S::RB; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) blocks[r][i] -= (float)(T)blocks[r][i];
+          rest[o] = to_operand<T>(blocks);
+        }
       }
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) {
         const u4 f = columns_fragment<T, DP>(columns + S::BYTES, st, d);
 #pragma unroll
-        for (int o = 0; o < OT; ++o) acc[d][o] = Mma<T>::step(f, pf[o], acc[d][o]);
+        for (int o = 0; o < OT; ++o) {
+          acc[d][o] = Mma<T>::step(f, pf[o], acc[d][o]);
+          if constexpr (BOTH) acc[d][o] = Mma<T>::step(f, rest[o], acc[d][o]);
+        }
       }
     }
   }
@@ -912,6 +927,15 @@ static bool pieces_ok(const View& v, size_t es) {
 }
 #define MIA_ATT_ONE(kernel, dp, ot, grid) \
   hipLaunchKernelGGL((kernel<T, dp, ot, decltype(dma)::value>), dim3((unsigned)(grid)), dim3(256), 0, s, a)
+#define MIA_ATT_FORWARD(dp, ot, both) \
+  hipLaunchKernelGGL((att_fwd_kernel<T, dp, ot, decltype(dma)::value, both>), dim3((unsigned)grid), dim3(256), 0, s, a)
+#define MIA_ATT_LAUNCH_FORWARD(ot, both)                  \
+  do {                                                    \
+    if (a.dim <= 32) MIA_ATT_FORWARD(32, ot, both);       \
+    else if (a.dim <= 64) MIA_ATT_FORWARD(64, ot, both);  \
+    else if (a.dim <= 96) MIA_ATT_FORWARD(96, ot, both);  \
+    else MIA_ATT_FORWARD(128, ot, both);                  \
+  } while (0)
 #define MIA_ATT_LAUNCH(kernel, ot, grid)                 \
   do {                                                   \
     if (a.dim <= 32) MIA_ATT_ONE(kernel, 32, ot, grid);  \
@@ -935,8 +959,10 @@ int Ops<T>::forward(Args a, hipStream_t s) {
   if (rc != MIA_OK) return rc;
   const bool dma = a.dim % (16 / (int)sizeof(T)) == 0 && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T));
   with_dma(dma, [&](auto dma) { 
-    if (pl.own_blocks == 2) MIA_ATT_LAUNCH(att_fwd_kernel, 2, grid);
-    else MIA_ATT_LAUNCH(att_fwd_kernel, 1, grid);
+    constexpr bool rounds = sizeof(T) == 2;  // (float: p is not rounded)
+    if (pl.own_blocks == 2) MIA_ATT_LAUNCH_FORWARD(2, false);
+    else if (pl.own_tiles == 1 && rounds) MIA_ATT_LAUNCH_FORWARD(1, rounds);
+    else MIA_ATT_LAUNCH_FORWARD(1, false);
   });
   if (a.splits > 1) {
     const long long rows = (long long)a.batch * a.heads * a.sq;
