@@ -288,10 +288,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // instead of three: 157 -> 140.  4 x 2048, 16 heads of 128: 148 us (927).  One query on 1500 keys, 16 items, 20 heads:
 // 26 us with the join, HBM.
 // BOTH: what the rounding of p to a two-byte type takes away goes through a second product, and the error falls from
-// 1.39 to 1.00 of a result rounded once.  For calls whose rows (up to 64 of a pair) fit one workgroup, as a decoding
-// step's do: memory sets their time and the matrix units are idle (16 x 1 on
-// 1500 keys, 20 heads of 64: 26.8 -> 26.9 us; 4 x 1 on 4096, 32 heads over 4 of 128: 27.7 -> 28.4; 1 x 1: 12.0 -> 12.4).  Not with more rows, where it costs
-// 7 - 20 % (1 x 1500, 20 heads of 64: 40 -> 46 us).
+// 1.39 to 1.00 of a result rounded once.  For calls whose rows (up to 64 of a pair) fit one workgroup: memory sets
+// their time and the matrix units are mostly idle (16 x 1 on 1500 keys, 20 heads of 64: 26.8 -> 26.9 us; 16 x 64:
+// 39.7 -> 41.8; 8 x 48 on 448, 6 heads: 10.4 -> 11.0).  Not with more rows, where it costs 7 - 20 % (1 x 1500,
+// 20 heads of 64: 40 -> 46 us).
 template <class T, int DP, int OT, bool DMA, bool BOTH>
 __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_fwd_kernel(att::Args p) {
   using namespace att;
@@ -728,7 +728,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     const int h = kvh * group + t / per_head, q0 = first + t % per_head * S::TILE;
     const unsigned at = lds0 + (t & 1) * 2 * S::BYTES;
     lq.issue(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.s, q0, p.sq, p.dim, at, wv, lane);
-    lg.issue(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.s, q0, p.sq, p.dim, at + S::BYTES, wv, lane);
+    lg.issue(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.s, q0, p.sq, p.dim, at + S::BYTES, wv,
+             lane);
     const bool in = lane < S::TILE && q0 + lane < p.sq;
     const float* from = p.stats + ((long long)b * p.heads + h) * p.sq + q0 + lane;
     if (wv == 0) dma4(in ? from : kInfinity, (unsigned)__builtin_amdgcn_readfirstlane((int)(lse_at + (t & 1) * 256u)));

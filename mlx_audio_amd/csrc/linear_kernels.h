@@ -483,7 +483,8 @@ struct Part {
 
 // Four waves, one tile per workgroup; several workgroups share a compute unit and fill each other's
 // gaps (dW of 24000 x 1280 -> 5120, bfloat16: 334 us here, 352 with the 256 tile in two parts; float32,
-// 6000 x 5120 -> 1280: 600 us, 131 TFLOP/s).  DMA: every 16-byte piece of both operands is aligned (bases, row strides) and lies either
+// 6000 x 5120 -> 1280: 600 us, 131 TFLOP/s).
+// DMA: every 16-byte piece of both operands is aligned (bases, row strides) and lies either
 // wholly inside its operand or wholly outside; otherwise pieces go through registers, element by
 // element at the edges.
 template <class TL, class T, bool AKC, bool BKC, bool DMA>
@@ -732,7 +733,8 @@ __global__ __launch_bounds__(64 * NW) void lin_few_kernel(lin::Gemm p) {
 
 // dz = dy act'(z), rounded to the operands' type for the two products that read it, and the column
 // sums of the unrounded values: workgroup (x, y) takes rows y, y + gridDim.y ... of 64 pieces of 16
-// bytes, four rows at a time (one per wave).  24000 x 5120, bfloat16: 150 us, 4.9 TB/s.  z null: no activation, sums only (dz null too).
+// bytes, four rows at a time (one per wave).  24000 x 5120, bfloat16: 150 us, 4.9 TB/s.
+// z null: no activation, sums only (dz null too).
 template <class T>
 __global__ __launch_bounds__(256) void lin_dz_kernel(const T* __restrict__ dy, long long dy_stride,
                                                      const T* __restrict__ z, long long z_stride, int act, int m,

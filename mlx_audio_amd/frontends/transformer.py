@@ -331,8 +331,8 @@ def attention(q, k, v, causal: bool = False, key_lengths=None, scale=None, retur
     Returns out [B, Sq, H, D], contiguous; with return_lse also the logarithm of each row's sum of
     exponentials, float32 [B, H, Sq] (-inf where no key is seen), which `attention_backward` takes.
     Few queries over many keys (a decoding step) are split along the keys and joined.  The
-    probabilities of two-byte types are rounded to that type for the product with v, except where
-    up to 64 rows share a key head (queries x heads per key head): those lose nothing.
+    probabilities of two-byte types are rounded to that type for the product with v, except with at
+    most 64 queries: those lose nothing.
     """
     ops = _operands(q=q, k=k, v=v)
     _same_type(ops, ("q", "k", "v"))
