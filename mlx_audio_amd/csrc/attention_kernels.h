@@ -135,6 +135,17 @@ __device__ __forceinline__ u4 to_operand(const f4* blocks) {
   }
 }
 
+// what the rounding to T took away
+template <class T, int RB>
+__device__ __forceinline__ u4 rest_operand(const f4* blocks) {
+  f4 rest[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rest[r][i] = blocks[r][i] - (float)(T)blocks[r][i];
+  return to_operand<T>(rest);
+}
+
 // Loads tiles of stream rows; rows at or past `end` read as zero whatever memory holds there, and so
 // do elements past dim through registers.  DMA: straight into LDS (pieces aligned, dim a whole
 // number of them); a place is then a uniform base plus a fixed offset per lane, and pieces past dim
@@ -442,13 +453,7 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
 #pragma unroll
         for (int r = 0; r < S::RB; ++r) blocks[r] = s[st * S::RB + r][o];
         pf[o] = to_operand<T>(blocks);
-        if constexpr (BOTH) {
-#pragma unroll
-          for (int r = 0; r < S::RB; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) blocks[r][i] -= (float)(T)blocks[r][i];
-          rest[o] = to_operand<T>(blocks);
-        }
+        if constexpr (BOTH) rest[o] = rest_operand<T, S::RB>(blocks);
       }
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) {
@@ -520,7 +525,11 @@ __global__ __launch_bounds__(256) void att_join_kernel(att::Args p) {
 
 // dq: own rows are queries, k and v stream.  Runs first and leaves for dk / dv what each query needs there:
 // stats[0] = lse / ln 2 (+inf for an empty row: its p becomes 0), stats[1] = delta = sum_d dout out.
-template <class T, int DP, int OT, bool DMA>
+// BOTH: as in the forward, for ds and up to 64 queries; the error of dq falls from 1.38 - 1.50 (float16, whose small
+// ds lose most) to 1.00 - 1.04 of a result rounded once.  The whole backward pass: 1 x 3662 keys 16.5 -> 17.9 us,
+// 16 x 1 on 1500, 20 heads of 64: 86 -> 89, 16 x 64: 94 -> 101.  dk / dv keep one part (1.41): with two they would have
+// to work on one block of keys per wave (16 x 1: 86 -> 106 us).
+template <class T, int DP, int OT, bool DMA, bool BOTH>
 __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   using namespace att;
   using S = Shape<T, DP>;
@@ -644,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
             for (int i = 0; i < 4; ++i)
               s[r][o][i] = k0 + 16 * (st * S::RB + r) + 4 * g + i < limit[o] ? s[r][o][i] : -kInf;
       }
-      u4 df[OT];
+      u4 df[OT], rest[OT];
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
         f4 blocks[S::RB];
@@ -655,12 +664,16 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
             blocks[r][i] = exp2_fast(fmaf(s[r][o][i], c, -lse2[o])) * dp[r][o][i];
           }
         df[o] = to_operand<T>(blocks);
+        if constexpr (BOTH) rest[o] = rest_operand<T, S::RB>(blocks);
       }
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) {
         const u4 f = columns_fragment<T, DP>(columns, st, d);
 #pragma unroll
-        for (int o = 0; o < OT; ++o) acc[d][o] = Mma<T>::step(f, df[o], acc[d][o]);
+        for (int o = 0; o < OT; ++o) {
+          acc[d][o] = Mma<T>::step(f, df[o], acc[d][o]);
+          if constexpr (BOTH) acc[d][o] = Mma<T>::step(f, rest[o], acc[d][o]);
+        }
       }
     }
   }
@@ -862,6 +875,7 @@ constexpr int kCus = 256;
 struct Plan {
   int pack, own_tiles, splits, keys_per_split, own_blocks;
 };
+constexpr int kFewQueries = 64;  // with no more, two-byte p (forward) and ds (dq) go into their product in two parts
 // Queries: 128 per workgroup (32 per wave), or 64 where that leaves compute units without work; then
 // the keys are split until there are two workgroups per unit.
 static Plan plan_forward(long long batch, long long sq, long long sk, int heads, int kv_heads) {
@@ -926,23 +940,23 @@ static bool pieces_ok(const View& v, size_t es) {
   const long long n = (long long)(16 / es);
   return aligned16(v.p) && v.b % n == 0 && v.s % n == 0 && v.h % n == 0 && v.s * (long long)es < (1LL << 25);
 }
-#define MIA_ATT_ONE(kernel, dp, ot, grid) \
-  hipLaunchKernelGGL((kernel<T, dp, ot, decltype(dma)::value>), dim3((unsigned)(grid)), dim3(256), 0, s, a)
-#define MIA_ATT_FORWARD(dp, ot, both) \
-  hipLaunchKernelGGL((att_fwd_kernel<T, dp, ot, decltype(dma)::value, both>), dim3((unsigned)grid), dim3(256), 0, s, a)
-#define MIA_ATT_LAUNCH_FORWARD(ot, both)                  \
-  do {                                                    \
-    if (a.dim <= 32) MIA_ATT_FORWARD(32, ot, both);       \
-    else if (a.dim <= 64) MIA_ATT_FORWARD(64, ot, both);  \
-    else if (a.dim <= 96) MIA_ATT_FORWARD(96, ot, both);  \
-    else MIA_ATT_FORWARD(128, ot, both);                  \
+#define MIA_ATT_ONE(grid, kernel, ...) \
+  hipLaunchKernelGGL((kernel<T, __VA_ARGS__>), dim3((unsigned)(grid)), dim3(256), 0, s, a)
+#define MIA_ATT_LAUNCH(grid, kernel, ot, ...)                                                  \
+  do {                                                                                         \
+    if (a.dim <= 32) MIA_ATT_ONE(grid, kernel, 32, ot, decltype(dma)::value __VA_ARGS__);      \
+    else if (a.dim <= 64) MIA_ATT_ONE(grid, kernel, 64, ot, decltype(dma)::value __VA_ARGS__); \
+    else if (a.dim <= 96) MIA_ATT_ONE(grid, kernel, 96, ot, decltype(dma)::value __VA_ARGS__); \
+    else MIA_ATT_ONE(grid, kernel, 128, ot, decltype(dma)::value __VA_ARGS__);                 \
   } while (0)
-#define MIA_ATT_LAUNCH(kernel, ot, grid)                 \
-  do {                                                   \
-    if (a.dim <= 32) MIA_ATT_ONE(kernel, 32, ot, grid);  \
-    else if (a.dim <= 64) MIA_ATT_ONE(kernel, 64, ot, grid); \
-    else if (a.dim <= 96) MIA_ATT_ONE(kernel, 96, ot, grid); \
-    else MIA_ATT_ONE(kernel, 128, ot, grid);             \
+#define MIA_ATT_COMMA ,
+// forward and dq: one block of queries a wave with both parts of p or ds, or without
+#define MIA_ATT_LAUNCH_QUERIES(grid, kernel, blocks)                                                     \
+  do {                                                                                                   \
+    constexpr bool rounds = sizeof(T) == 2; /* (float: nothing is rounded) */                            \
+    if (blocks == 2) MIA_ATT_LAUNCH(grid, kernel, 2, MIA_ATT_COMMA false);                               \
+    else if (rounds && a.sq <= kFewQueries) MIA_ATT_LAUNCH(grid, kernel, 1, MIA_ATT_COMMA rounds);       \
+    else MIA_ATT_LAUNCH(grid, kernel, 1, MIA_ATT_COMMA false);                                           \
   } while (0)
 
 template <class F>
@@ -960,10 +974,7 @@ int Ops<T>::forward(Args a, hipStream_t s) {
   if (rc != MIA_OK) return rc;
   const bool dma = a.dim % (16 / (int)sizeof(T)) == 0 && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T));
   with_dma(dma, [&](auto dma) { 
-    constexpr bool rounds = sizeof(T) == 2;  // (float: p is not rounded)
-    if (pl.own_blocks == 2) MIA_ATT_LAUNCH_FORWARD(2, false);
-    else if (pl.own_tiles == 1 && rounds) MIA_ATT_LAUNCH_FORWARD(1, rounds);
-    else MIA_ATT_LAUNCH_FORWARD(1, false);
+    MIA_ATT_LAUNCH_QUERIES(grid, att_fwd_kernel, pl.own_blocks);
   });
   if (a.splits > 1) {
     const long long rows = (long long)a.batch * a.heads * a.sq;
@@ -992,8 +1003,7 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
     a.own_tiles = of_dq.own_tiles, a.splits = of_dq.splits;
     a.o0 = dq, a.o1 = nullptr;
     with_dma(whole && pieces_ok(a.k, sizeof(T)) && pieces_ok(a.v, sizeof(T)), [&](auto dma) {
-      if (of_dq.own_blocks == 2) MIA_ATT_LAUNCH(att_dq_kernel, 2, dq_grid);
-      else MIA_ATT_LAUNCH(att_dq_kernel, 1, dq_grid);
+      MIA_ATT_LAUNCH_QUERIES(dq_grid, att_dq_kernel, of_dq.own_blocks);
     });
     if (a.splits > 1) add(rows * a.dim, rows * a.dim, dq, nullptr);
   }
@@ -1003,13 +1013,13 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
     with_dma(whole && pieces_ok(a.q, sizeof(T)) && pieces_ok(a.dout, sizeof(T)), [&](auto dma) {
       if (of_dkv.own_blocks == 2) {
         if constexpr (sizeof(T) == 2) {
-          if (a.dim <= 32) MIA_ATT_ONE(att_dkv_kernel, 32, 2, dkv_grid);
-          else MIA_ATT_ONE(att_dkv_kernel, 64, 2, dkv_grid);
+          if (a.dim <= 32) MIA_ATT_ONE(dkv_grid, att_dkv_kernel, 32, 2, decltype(dma)::value);
+          else MIA_ATT_ONE(dkv_grid, att_dkv_kernel, 64, 2, decltype(dma)::value);
         } else {
-          MIA_ATT_ONE(att_dkv_kernel, 32, 2, dkv_grid);
+          MIA_ATT_ONE(dkv_grid, att_dkv_kernel, 32, 2, decltype(dma)::value);
         }
       } else {
-        MIA_ATT_LAUNCH(att_dkv_kernel, 1, dkv_grid);
+        MIA_ATT_LAUNCH(dkv_grid, att_dkv_kernel, 1, );
       }
     });
     if (a.splits > 1) {
