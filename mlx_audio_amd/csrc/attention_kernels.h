@@ -741,8 +741,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     const int h = kvh * group + t / per_head, q0 = first + t % per_head * S::TILE;
     const unsigned at = lds0 + (t & 1) * 2 * S::BYTES;
     lq.issue(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.s, q0, p.sq, p.dim, at, wv, lane);
-    lg.issue(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.s, q0, p.sq, p.dim, at + S::BYTES, wv,
-             lane);
+    lg.issue(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.s, q0, p.sq, p.dim, at + S::BYTES,
+             wv, lane);
     const bool in = lane < S::TILE && q0 + lane < p.sq;
     const float* from = p.stats + ((long long)b * p.heads + h) * p.sq + q0 + lane;
     if (wv == 0) dma4(in ? from : kInfinity, (unsigned)__builtin_amdgcn_readfirstlane((int)(lse_at + (t & 1) * 256u)));
