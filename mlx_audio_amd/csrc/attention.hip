@@ -74,7 +74,7 @@ int mia_attention(const mia_attention_desc* d, const void* q, const void* k, con
 
 size_t mia_attention_backward_workspace_bytes(const mia_attention_desc* d) {
   if (att::check(d) != MIA_OK) return 0;
-  return att::gradient_bytes(d->batch, d->queries, d->keys, d->heads, d->kv_heads, d->dim, nn::dtype_size(d->dtype));
+  return att::gradient_bytes(d->batch, d->queries, d->keys, d->heads, d->kv_heads, d->dim, d->dtype);
 }
 
 int mia_attention_backward(const mia_attention_desc* d, const void* dout, const int64_t* stride_dout, const void* q,

@@ -16,6 +16,10 @@
 // LDS down the columns (ds_read_b64_tr_b16; float: ds_read_b32).  Row maxima and sums need two lane
 // exchanges.  dk / dv and dq are two launches: one launch would need atomics for dq, whose order
 // changes its bits.
+//
+// float16 has too few exponents for the gradients' p and ds as they are (1500 keys: p is about 2^-11, ds
+// less by the size of dout, and below 2^-14 float16 loses bits).  They go into their products times
+// powers of two, taken out again in float32 when the result is stored: Scale and att_range_kernel.
 #pragma once
 #include "nn_common.h"
 
@@ -33,7 +37,9 @@ struct Args {
   void* o1;           // dv
   float* lse;         // (batch, heads, sq): written by the forward, read by the backward
   float* stats;       // backward: lse / ln 2 (+inf for an empty row), then delta, (batch, heads, sq) each;
-                      // dq writes them, dk / dv reads them
+                      // dq writes them, dk / dv reads them; float16: with dk / dv's Scale in them
+  float* range;       // float16 gradients: (batch, kv_heads, range_parts, 2) bounds of the norms of v and dout
+  int range_parts;
   const int* lengths; // (batch) keys of each batch item, or null
   int batch, sq, sk, heads, kv_heads, dim;
   int pack;           // heads that share a workgroup's rows: 1, or heads / kv_heads (few queries)
@@ -291,7 +297,59 @@ __device__ __forceinline__ float column_sum(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
 }
+// a value that all lanes share, in a scalar register
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Powers of two that p and dp - delta are taken times, so that ds = p (dp - delta) fills float16's range:
+// |dp - delta| <= |dout| (|v| + |out|) <= 2 |dout| max |v|, a row's out being a mean of values, so ds times
+// 2^(p + dp) with the largest power that keeps that bound below 2^14 cannot overflow; p itself, at most 1,
+// takes at most 2^14.  The factor of dp goes into its own operand, dout in dq and v in dk / dv (rounded there
+// only where it is less than 1, and then by less than 2^-17 of the largest), and into delta.
+struct Scale {
+  int p, dp;
+};
+__device__ __forceinline__ int above(float x) {  // the least e with x < 2^e; x not below 2^-60
+  return __builtin_amdgcn_frexp_expf(fmaxf(x, 0x1p-60f));
+}
+// dq: own is |dout| of a row, other the largest |v|.  Only ds meets float16 there: p takes what dp cannot.
+__device__ __forceinline__ Scale dq_scale(float own, float other) {
+  const float bound = 2.0f * own * other;
+  if (!(bound < kInf)) return {0, 0};
+  const int room = 14 - above(bound);
+  const int p = min(room, 14);
+  return {p, max(0, min(min(room - p, 14 - above(own)), 14))};
+}
+// dk / dv: own is the largest |v|, other the largest |dout|.  p is dv's operand as well: never less than itself.
+__device__ __forceinline__ Scale dkv_scale(float own, float other) {
+  const float bound = 2.0f * own * other;
+  if (!(bound < kInf)) return {0, 0};
+  const int room = 14 - above(bound);
+  const int p = max(0, min(room, 14));
+  return {p, min(min(room - p, max(0, 14 - above(own))), 14)};
+}
+// bounds of the norms of a key head's values (x) and of its query heads' dout rows (y)
+__device__ __forceinline__ float2 norms_of(const Args& p, int b, int kvh) {
+  const float* from = p.range + ((long long)b * p.kv_heads + kvh) * p.range_parts * 2;
+  float2 most = {0.0f, 0.0f};
+  for (int i = 0; i < p.range_parts; ++i) most.x = fmaxf(most.x, from[2 * i]), most.y = fmaxf(most.y, from[2 * i + 1]);
+  return most;
+}
+// an own row's vector times 2^e
+template <class T, int N>
+__device__ __forceinline__ void scale_own(u4 (&v)[N], int e) {
+  const float f = exp2_fast((float)e);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float x[kPer16<T>];
+    unpack<T>(v[i], x);
+#pragma unroll
+    for (int j = 0; j < kPer16<T>; ++j) x[j] *= f;
+    v[i] = pack<T>(x);
+  }
+}
 }  // namespace att
 
 // Forward.  OT: blocks of 16 queries per wave.  bfloat16, 8 x 1500, 20 heads of 64: 139 us (663 TFLOP/s), bound by the
@@ -523,10 +581,61 @@ __global__ __launch_bounds__(256) void att_join_kernel(att::Args p) {
   if (lane == 0 && p.lse) p.lse[at] = total == 0.0f ? -kInf : fmaf(top, kLn2, logf(total));
 }
 
+// Bounds of the norms of a key head's v rows and of the dout rows of its query heads, over 1 / range_parts of
+// them: 16 lanes a row, each with the largest sum of squares of its own 16 bytes over all rows; added up at
+// the end they are at least the largest norm's square, and no row waits for an exchange of lanes.  Reads both once:
+// 8 x 1500, 20 heads of 64: 15 us (61 MB, HBM) of a backward pass of 391; 16 x 1 on 1500: 15 of 102; 2 x 100, 6 heads: 3
+// of 29.  What it buys: 1.7 - 4.7 times the error of a result rounded once, with dout of 1e-2 ... 1e-5, become 1.4.
+template <class T>
+__global__ __launch_bounds__(256) void att_range_kernel(att::Args p) {
+  using namespace att;
+  constexpr int V = kPer16<T>, AHEAD = 8;
+  __shared__ float red[4][2];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int part = (int)(blockIdx.x % (unsigned)p.range_parts), pair = (int)(blockIdx.x / (unsigned)p.range_parts);
+  const int kvh = pair % p.kv_heads, b = pair / p.kv_heads, group = p.heads / p.kv_heads;
+  const int e = (lane & 15) * V;
+  // rows of one head from `base` on, `count` of them
+  auto largest = [&](const T* base, long long stride, int count, float most) {
+    const int begin = (int)((long long)count * part / p.range_parts), end = (int)((long long)count * (part + 1) / p.range_parts);
+    for (int row0 = begin + (int)(threadIdx.x >> 4); row0 < end; row0 += 16 * AHEAD) {
+      u4 raw[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int row = row0 + 16 * i;
+        raw[i] = u4{0, 0, 0, 0};
+        if (row < end && e < p.dim)
+          raw[i] = load_piece(base + row * stride + e, p.dim - e, (count - 1 - row) * stride + p.dim - e);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        float x[V], s = 0.0f;
+        unpack<T>(raw[i], x);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s = fmaf(x[j], x[j], s);
+        most = fmaxf(most, s);
+      }
+    }
+    return most;
+  };
+  float v = largest(static_cast<const T*>(p.v.p) + b * p.v.b + kvh * p.v.h, p.v.s, keys_of(p, b), 0.0f), g = 0.0f;
+  for (int h = kvh * group; h < (kvh + 1) * group; ++h)
+    g = largest(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.s, p.sq, g);
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o)), g = fmaxf(g, __shfl_xor(g, o));
+#pragma unroll
+  for (int o = 8; o; o >>= 1) v += __shfl_xor(v, o), g += __shfl_xor(g, o);
+  if (lane == 0) red[wv][0] = v, red[wv][1] = g;
+  __syncthreads();
+  if (threadIdx.x < 2)
+    p.range[(long long)blockIdx.x * 2 + threadIdx.x] = sqrtf(fmaxf(
+        fmaxf(red[0][threadIdx.x], red[1][threadIdx.x]), fmaxf(red[2][threadIdx.x], red[3][threadIdx.x])));
+}
+
 // dq: own rows are queries, k and v stream.  Runs first and leaves for dk / dv what each query needs there:
 // stats[0] = lse / ln 2 (+inf for an empty row: its p becomes 0), stats[1] = delta = sum_d dout out.
-// BOTH: as in the forward, for ds and up to 64 queries; the error of dq falls from 1.38 - 1.50 (float16, whose small
-// ds lose most) to 1.00 - 1.04 of a result rounded once.  The whole backward pass: 1 x 3662 keys 16.5 -> 17.9 us,
+// BOTH: as in the forward, for ds and up to 64 queries; the error of dq falls from 1.38 - 1.50 to 1.00 - 1.04 of
+// a result rounded once.  The whole backward pass (bfloat16): 1 x 3662 keys 16.5 -> 17.9 us,
 // 16 x 1 on 1500, 20 heads of 64: 86 -> 89, 16 x 64: 94 -> 101.  dk / dv keep one part (1.41): with two they would have
 // to work on one block of keys per wave (16 x 1: 86 -> 106 us).
 template <class T, int DP, int OT, bool DMA, bool BOTH>
@@ -552,9 +661,13 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   const int open = p.causal ? min(len, row0 + off + 1) : len;
 
   const long long n = (long long)p.batch * p.heads * p.sq;
+  constexpr bool SCALED = std::is_same<T, _Float16>::value;
   u4 oq[OT][S::CC], og[OT][S::CC];
-  float lse2[OT], delta[OT];
+  float lse2[OT], delta[OT], factor[OT];
   int limit[OT];
+  float2 most = {0.0f, 0.0f};
+  Scale there = {0, 0};  // of dk / dv
+  if constexpr (SCALED) most = norms_of(p, b, kvh), there = dkv_scale(most.x, most.y);
 #pragma unroll
   for (int o = 0; o < OT; ++o) {
     const int s = row0 + 16 * o + (lane & 15);
@@ -566,22 +679,33 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
     u4 oo[S::CC];
     load_own<T, DP>(static_cast<const T*>(p.out.p) + b * p.out.b + s * p.out.s + h * p.out.h, in, p.dim,
                     (p.sq - 1 - s) * p.out.s, lane, oo);
-    float d = 0.0f;
+    float d = 0.0f, gg = 0.0f;
 #pragma unroll
     for (int cc = 0; cc < S::CC; ++cc) {
       float x[S::V], y[S::V];
       unpack<T>(oo[cc], x);
       unpack<T>(og[o][cc], y);
 #pragma unroll
-      for (int j = 0; j < S::V; ++j) d = fmaf(x[j], y[j], d);
+      for (int j = 0; j < S::V; ++j) {
+        d = fmaf(x[j], y[j], d);
+        if constexpr (SCALED) gg = fmaf(y[j], y[j], gg);
+      }
     }
     const long long at = ((long long)b * p.heads + h) * p.sq + s;
     const float l = in ? p.lse[at] : -kInf;
     delta[o] = column_sum(d);
     lse2[o] = l == -kInf ? kInf : l * kLog2e;
+    factor[o] = p.scale;
     if (in && g == 0 && split == 0) {
-      p.stats[at] = lse2[o];
-      p.stats[n + at] = delta[o];
+      p.stats[at] = SCALED ? lse2[o] - (float)there.p : lse2[o];
+      p.stats[n + at] = SCALED ? ldexpf(delta[o], there.dp) : delta[o];
+    }
+    if constexpr (SCALED) {
+      const Scale here = dq_scale(sqrtf(column_sum(gg)), most.x);
+      lse2[o] -= (float)here.p;
+      delta[o] = ldexpf(delta[o], here.dp);
+      scale_own<T>(og[o], here.dp);
+      factor[o] = ldexpf(p.scale, -here.p - here.dp);
     }
     limit[o] = p.causal ? min(len, s + off + 1) : len;
   }
@@ -682,8 +806,8 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
     const int s = row0 + 16 * o + (lane & 15);
     if (s >= p.sq) continue;
     const long long at = (((long long)b * p.sq + s) * p.heads + h) * p.dim;
-    if (p.splits > 1) store_own<float>(p.partial + split * n * p.dim + at, p.dim, lane, acc, o, p.scale);
-    else store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, acc, o, p.scale);
+    if (p.splits > 1) store_own<float>(p.partial + split * n * p.dim + at, p.dim, lane, acc, o, factor[o]);
+    else store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, acc, o, factor[o]);
   }
 }
 
@@ -717,6 +841,14 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
                     (p.sk - 1 - s) * p.k.s, lane, ok[o]);
     load_own<T, DP>(static_cast<const T*>(p.v.p) + b * p.v.b + (long long)s * p.v.s + kvh * p.v.h, s < len, p.dim,
                     (p.sk - 1 - s) * p.v.s, lane, ov[o]);
+  }
+  float of_dk = p.scale, of_dv = 1.0f;
+  if constexpr (std::is_same<T, _Float16>::value) {
+    const float2 most = norms_of(p, b, kvh);
+    const Scale sc = dkv_scale(most.x, most.y);
+    of_dk = uniform(ldexpf(p.scale, -sc.p - sc.dp)), of_dv = uniform(ldexpf(1.0f, -sc.p));
+#pragma unroll
+    for (int o = 0; o < OT; ++o) scale_own<T>(ov[o], sc.dp);
   }
   f4 dk[S::DT][OT], dv[S::DT][OT];
 #pragma unroll
@@ -848,11 +980,11 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
     const long long at = (((long long)b * p.sk + s) * p.kv_heads + kvh) * p.dim;
     if (p.splits > 1) {
       const long long count = (long long)p.batch * p.sk * p.kv_heads * p.dim;
-      store_own<float>(p.partial + 2 * split * count + at, p.dim, lane, dk, o, p.scale);
-      store_own<float>(p.partial + (2 * split + 1) * count + at, p.dim, lane, dv, o, 1.0f);
+      store_own<float>(p.partial + 2 * split * count + at, p.dim, lane, dk, o, of_dk);
+      store_own<float>(p.partial + (2 * split + 1) * count + at, p.dim, lane, dv, o, of_dv);
     } else {
-      store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, dk, o, p.scale);
-      store_own<T>(static_cast<T*>(p.o1) + at, p.dim, lane, dv, o, 1.0f);
+      store_own<T>(static_cast<T*>(p.o0) + at, p.dim, lane, dk, o, of_dk);
+      store_own<T>(static_cast<T*>(p.o1) + at, p.dim, lane, dv, o, of_dv);
     }
   }
 }
@@ -922,11 +1054,24 @@ static GradPlan plan_dkv(long long batch, long long sq, long long sk, int heads,
 static GradPlan plan_dq(long long batch, long long sq, long long sk, int heads, size_t es) {
   return plan_gradient(batch * heads, sq, stream_tiles(sk, es), true);
 }
-static size_t gradient_bytes(long long batch, long long sq, long long sk, int heads, int kv_heads, int dim, size_t es) {
+// Workgroups of a pair of att_range_kernel: four per compute unit, of at least 128 rows each.
+static int range_parts(long long batch, long long sq, long long sk, int heads, int kv_heads) {
+  const long long pairs = batch * kv_heads, rows = sk + sq * (heads / kv_heads);
+  long long parts = pairs ? (4 * kCus + pairs - 1) / pairs : 1;
+  if (parts > rows / 128) parts = rows / 128;
+  return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+}
+static size_t stats_bytes(long long rows) { return align256((size_t)2 * rows * sizeof(float)); }
+static size_t range_bytes(long long batch, int kv_heads, int parts) {
+  return align256((size_t)2 * batch * kv_heads * parts * sizeof(float));
+}
+static size_t gradient_bytes(long long batch, long long sq, long long sk, int heads, int kv_heads, int dim, int dtype) {
+  const size_t es = dtype_size(dtype);
   const GradPlan k = plan_dkv(batch, sq, sk, heads, kv_heads, dim, es), q = plan_dq(batch, sq, sk, heads, es);
   const size_t kb = k.splits > 1 ? (size_t)2 * k.splits * batch * sk * kv_heads * dim * sizeof(float) : 0;
   const size_t qb = q.splits > 1 ? (size_t)q.splits * batch * sq * heads * dim * sizeof(float) : 0;
-  return align256((size_t)2 * batch * heads * sq * sizeof(float)) + (kb > qb ? kb : qb);
+  const size_t range = dtype == MIA_F16 ? range_bytes(batch, kv_heads, range_parts(batch, sq, sk, heads, kv_heads)) : 0;
+  return stats_bytes(batch * heads * sq) + range + (kb > qb ? kb : qb);
 }
 
 template <class T>
@@ -993,7 +1138,15 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
   const int rc = check_grid(dq_grid > dkv_grid ? dq_grid : dkv_grid);
   if (rc != MIA_OK) return rc;
   a.stats = stats, a.pack = 1;
-  a.partial = stats + align256((size_t)2 * rows * sizeof(float)) / sizeof(float);
+  a.partial = stats + stats_bytes(rows) / sizeof(float);
+  if constexpr (std::is_same<T, _Float16>::value) {
+    a.range = a.partial, a.range_parts = range_parts(a.batch, a.sq, a.sk, a.heads, a.kv_heads);
+    a.partial += range_bytes(a.batch, a.kv_heads, a.range_parts) / sizeof(float);
+    const long long range_grid = (long long)a.batch * a.kv_heads * a.range_parts;  // (no more than dkv's, or 64 a pair)
+    const int fits = check_grid(range_grid);
+    if (fits != MIA_OK) return fits;
+    hipLaunchKernelGGL(att_range_kernel<T>, dim3((unsigned)range_grid), dim3(256), 0, s, a);
+  }
   auto add = [&](long long total, long long n, void* out0, void* out1) {
     const long long blocks = (total + 255) / 256;
     hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a.partial,

@@ -360,9 +360,9 @@ def attention_backward(dout, q, k, v, out, lse, causal: bool = False, key_length
     dout and out [B, Sq, H, D], lse float32 [B, H, Sq]; the other arguments as in the forward call.
     The probabilities are recomputed, nothing of size Sq x Sk is kept.  dk and dv are summed over the
     query heads that share a key head, and zero behind a length.  For the products the
-    probabilities and their gradients are rounded to the operands' type (not in dq with at most
-    64 queries): in float16 a gradient
-    of a score beyond 65504 becomes infinite (as a loss scaled too far should show).
+    probabilities and their gradients are rounded to the operands' type (in dq with at most 64
+    queries: carried in two parts); in float16 both are taken times powers of two first, worked out
+    from the largest norms of v and dout, so that they neither overflow nor lose bits by being small.
     """
     ops = _operands(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
     _same_type(ops, ("dout", "q", "k", "v", "out"))
