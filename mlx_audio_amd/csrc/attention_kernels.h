@@ -154,12 +154,14 @@ __device__ __forceinline__ u4 rest_operand(const f4* blocks) {
 
 // Loads tiles of stream rows; rows at or past `end` read as zero whatever memory holds there, and so
 // do elements past dim through registers.  DMA: straight into LDS (pieces aligned, dim a whole
-// number of them); a place is then a uniform base plus a fixed offset per lane, and pieces past dim
-// repeat the row's first one: the other operand is zero there, or the result is never stored.
+// number of them); a place is then a uniform base plus a fixed offset per lane.  Pieces between dim and DP
+// stay as `clear` leaves them, zero: the other operand is zero there, and anything else might be infinite.
+// Pieces from DP on are never read; where dim is DP, they repeat the row's first one.
 template <class T, int DP, bool DMA>
 struct Loader {
   using S = Shape<T, DP>;
   unsigned offset[S::PW];
+  unsigned long long lanes[S::PW];  // that load
   u4 held[DMA ? 1 : S::PW];
   static __device__ __forceinline__ void where(int i, int wv, int lane, int& r, int& c) {
     const int s = (S::PW * wv + i) * 64 + lane;
@@ -171,6 +173,20 @@ struct Loader {
       int r, c;
       where(i, wv, lane, r, c);
       offset[i] = (unsigned)((r * stride + (c * S::V < dim ? c * S::V : 0)) * S::ES);
+      lanes[i] = __ballot(dim == DP || c * S::V < dim);
+    }
+  }
+  // Zeros past dim in both buffers of a tile, before the first load into them.
+  static __device__ __forceinline__ void clear(unsigned char* tile, int dim, int wv, int lane) {
+    if constexpr (DMA) {
+      if (dim == DP) return;
+#pragma unroll
+      for (int i = 0; i < S::PW; ++i) {
+        int r, c;
+        where(i, wv, lane, r, c);
+        unsigned char* at = tile + ((S::PW * wv + i) * 64 + lane) * 16;
+        if (c * S::V >= dim) *reinterpret_cast<u4*>(at) = *reinterpret_cast<u4*>(at + 2 * S::BYTES) = u4{0, 0, 0, 0};
+      }
     }
   }
   __device__ __forceinline__ void issue(const void* base, long long stride, int row0, int end, int dim, unsigned lds,
@@ -180,13 +196,13 @@ struct Loader {
       const unsigned dst = (unsigned)__builtin_amdgcn_readfirstlane((int)(lds + (unsigned)(S::PW * wv) * 1024u));
       if (row0 + S::TILE <= end) {
 #pragma unroll
-        for (int i = 0; i < S::PW; ++i) dma16(from, offset[i], dst + 1024u * i);
+        for (int i = 0; i < S::PW; ++i) dma16(from, offset[i], dst + 1024u * i, lanes[i]);
       } else {
 #pragma unroll
         for (int i = 0; i < S::PW; ++i) {
           int r, c;
           where(i, wv, lane, r, c);
-          dma16(row0 + r < end ? from + offset[i] : reinterpret_cast<const char*>(kZeros), dst + 1024u * i);
+          dma16(row0 + r < end ? from + offset[i] : reinterpret_cast<const char*>(kZeros), dst + 1024u * i, lanes[i]);
         }
       }
     } else {
@@ -427,6 +443,8 @@ __global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 128 ? 4 : 2) void att_f
   Loader<T, DP, DMA> lk, lv;
   lk.init(p.k.s, p.dim, wv, lane);
   lv.init(p.v.s, p.dim, wv, lane);
+  lk.clear(smem, p.dim, wv, lane);
+  lv.clear(smem + S::BYTES, p.dim, wv, lane);
   const int tiles = k_end > k_begin ? (k_end - k_begin + S::TILE - 1) / S::TILE : 0;
   if (tiles) {
     lk.issue(kp, p.k.s, k_begin, k_end, p.dim, lds0, wv, lane);
@@ -722,6 +740,8 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
   Loader<T, DP, DMA> lk, lv;
   lk.init(p.k.s, p.dim, wv, lane);
   lv.init(p.v.s, p.dim, wv, lane);
+  lk.clear(smem, p.dim, wv, lane);
+  lv.clear(smem + S::BYTES, p.dim, wv, lane);
   const int all = k_end > 0 ? (k_end + S::TILE - 1) / S::TILE : 0;
   const int begin = (int)((long long)all * split / p.splits), end = (int)((long long)all * (split + 1) / p.splits);
   if (begin < end) {
@@ -869,6 +889,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   Loader<T, DP, DMA> lq, lg;
   lq.init(p.q.s, p.dim, wv, lane);
   lg.init(p.dout.s, p.dim, wv, lane);
+  lq.clear(smem, p.dim, wv, lane);
+  lg.clear(smem + S::BYTES, p.dim, wv, lane);
   auto issue = [&](int t) {
     const int h = kvh * group + t / per_head, q0 = first + t % per_head * S::TILE;
     const unsigned at = lds0 + (t & 1) * 2 * S::BYTES;

@@ -156,6 +156,30 @@ __device__ __forceinline__ void dma16(const void* base, unsigned offset, unsigne
       : "s"(base), "v"(offset), "s"(lds_byte_addr)
       : "memory", "m0");
 }
+// either, of the lanes in `lanes` only; the others' places stay as they are
+__device__ __forceinline__ void dma16(const void* base, unsigned offset, unsigned lds_byte_addr,
+                                      unsigned long long lanes) {
+  unsigned long long active;
+  asm volatile(
+      "s_mov_b32 m0, %3\n\t"
+      "s_and_saveexec_b64 %0, %4\n\t"
+      "global_load_lds_dwordx4 %2, %1\n\t"
+      "s_mov_b64 exec, %0"
+      : "=&s"(active)
+      : "s"(base), "v"(offset), "s"(lds_byte_addr), "s"(lanes)
+      : "memory", "m0", "scc");
+}
+__device__ __forceinline__ void dma16(const void* gptr, unsigned lds_byte_addr, unsigned long long lanes) {
+  unsigned long long active;
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_and_saveexec_b64 %0, %3\n\t"
+      "global_load_lds_dwordx4 %1, off\n\t"
+      "s_mov_b64 exec, %0"
+      : "=&s"(active)
+      : "v"(gptr), "s"(lds_byte_addr), "s"(lanes)
+      : "memory", "m0", "scc");
+}
 #pragma clang diagnostic pop
 // the same with 4 bytes a lane, at lds_byte_addr + 4 L
 __device__ __forceinline__ void dma4(const void* gptr, unsigned lds_byte_addr) {
