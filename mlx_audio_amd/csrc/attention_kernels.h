@@ -999,6 +999,10 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_ker
   for (int o = 0; o < OT; ++o) {
     const int s = row0 + 16 * o + (lane & 15);
     if (s >= p.sk) continue;
+    if (s >= len) {  // zero whatever dout holds (0 x inf in the sums would not be)
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) dk[d][o] = dv[d][o] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     const long long at = (((long long)b * p.sk + s) * p.kv_heads + kvh) * p.dim;
     if (p.splits > 1) {
       const long long count = (long long)p.batch * p.sk * p.kv_heads * p.dim;

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from mlx_audio_amd.frontends import attention
+from mlx_audio_amd.frontends import attention, attention_backward
 from test_gpu_attention import TYPES, bounds, close, f64, make, u
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +43,22 @@ def test_infinite_values_stay_in_their_columns(gpu, t, dim):
     assert (out[0, :, 1, 2] == float("inf")).all()
     out[0, :, 1, 2] = want[0, :, 1, 2]
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("sq", [5, 300])
+def test_gradients_behind_a_length_are_zero_whatever_dout_holds(gpu, t, bad, sq):
+    t = TYPES[t]
+    lengths = [1, 37, 64, 65, 150, 0]
+    q, k, v = make((6, sq, 4, 64), t, 7), make((6, 150, 2, 64), t, 8), make((6, 150, 2, 64), t, 9)
+    dout = make(q.shape, t, 10)
+    out, lse = attention(q, k, v, key_lengths=lengths, return_lse=True)
+    good = attention_backward(dout, q, k, v, out, lse, key_lengths=lengths)
+    dout[:, sq // 2, 1, 3] = bad
+    got = attention_backward(dout, q, k, v, out, lse, key_lengths=lengths)
+    for b, n in enumerate(lengths):
+        assert all((g[b, n:] == 0).all() for g in got[1:]), b
+    # the query's own row of dq and its key head are spoilt, nothing else (float16: but for the scale)
+    assert torch.equal(got[0][:, :, 2:], good[0][:, :, 2:]) if t != torch.float16 else torch.isfinite(got[0][:, :, 2:]).all()
+    assert all(torch.isfinite(g[:, :, 1]).all() for g in got[1:])
