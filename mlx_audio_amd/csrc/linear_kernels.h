@@ -40,21 +40,26 @@ struct Gemm {
   Epilogue e;
 };
 
-// 0.5 erfc(-x / sqrt 2) from erfc(z) = t (a1 + t (a2 + ... a5 t)) exp(-z^2), t = 1 / (1 + p z)
-// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26):
-// absolute error 1.5e-7 and no cancellation in the negative tail; `e` receives exp(-x^2 / 2).
+// 0.5 erfc(-x / sqrt 2) from erfc(z) = t (a1 + t (a2 + ... t a7)) exp(-z^2), t = 1 / (1 + 0.51 z): the
+// coefficients are the least relative error (7.2e-7) over 0 <= z <= 9.4, behind which the result is below
+// 1e-38, found by reweighted least squares against erfc(z) exp(z^2).  So x Phi(x) keeps its digits in the
+// negative tail; the exponent's argument, rounded three times, adds at most 1.5e-5 there (x = -12.9).
+// `e` receives exp(-x^2 / 2).
 __device__ __forceinline__ float normal_cdf_fast(float x, float& e) {
   const float z = __builtin_fabsf(x) * 0.70710678118654752440f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-  float q = fmaf(t, 1.061405429f, -1.453152027f);
-  q = fmaf(t, q, 1.421413741f);
-  q = fmaf(t, q, -0.284496736f);
-  q = fmaf(t, q, 0.254829592f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.51f, z, 1.0f));
+  float q = fmaf(t, 0.09548515f, -0.3624904f);
+  q = fmaf(t, q, 0.36299136f);
+  q = fmaf(t, q, 0.05193581f);
+  q = fmaf(t, q, 0.28020033f);
+  q = fmaf(t, q, 0.28394583f);
+  q = fmaf(t, q, 0.28793213f);
   e = __builtin_amdgcn_exp2f(-1.44269504088896340736f * z * z);
   const float half_erfc = 0.5f * t * q * e;
   return x < 0.0f ? half_erfc : 1.0f - half_erfc;
 }
-// Two-byte results: the polynomial's 1.5e-7 is far below their rounding.  float: the library's erfc.
+// Two-byte results: 1.5e-5 of a value and less is far below their rounding (2^-12 of it at the least).  float: the
+// library's erfc.
 template <bool PRECISE>
 __device__ __forceinline__ float activate(float z, int act) {
   if (act == MIA_ACT_GELU) {
