@@ -77,6 +77,9 @@ __device__ __forceinline__ float activate(float z, int act) {
 }
 template <bool PRECISE>
 __device__ __forceinline__ float derivative(float z, int act) {
+  // at +-20 either GELU's slope is 0 or 1 exactly; the limit keeps z exp(-z^2 / 2) and z^3 from infinities (a
+  // float16 preactivation is one beyond 65504) and a NaN a NaN
+  if (act == MIA_ACT_GELU || act == MIA_ACT_GELU_TANH) z = z > 20.0f ? 20.0f : (z < -20.0f ? -20.0f : z);
   if (act == MIA_ACT_GELU) {
     float e, cdf;
     if constexpr (PRECISE) {
@@ -88,8 +91,6 @@ __device__ __forceinline__ float derivative(float z, int act) {
     return fmaf(z * 0.39894228040143267794f, e, cdf);
   }
   if (act == MIA_ACT_GELU_TANH) {
-    // at +-20 the slope is 0 or 1 exactly; the limit keeps z^3 finite (and a NaN a NaN)
-    z = z > 20.0f ? 20.0f : (z < -20.0f ? -20.0f : z);
     const float u2 = 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
     const float s = 1.0f / (1.0f + expf(-u2));
     return fmaf(z * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), s);

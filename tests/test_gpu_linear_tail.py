@@ -45,3 +45,23 @@ def test_gelu_derivative(gpu, t):
     err = np.abs(f64(dx) - want)
     assert (err <= tol).all(), (np.max(err / tol), zd.flat[np.argmax(err / tol)])
     assert (np.abs(f64(db) - want.sum(0)) <= (REL + 700 * 2.0 ** -24) * size.sum(0)).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "relu"])
+def test_slope_at_infinite_preactivations(gpu, t, act):
+    """What the forward call keeps may be infinite (float16: beyond 65504) where its result is not: the slope
+    there is the limit, 0 or 1."""
+    t = TYPES[t]
+    inf = float("inf")
+    z = torch.tensor([[-inf, inf, -6e4, 6e4, float("nan")]], device="cuda").to(t)
+    eye = torch.eye(5, dtype=t, device="cuda")
+    db = linear_backward(torch.ones_like(z), z[:, :5], eye, activation=act, preactivation=z, input_grad=False,
+                         weight_grad=False)[2]
+    assert db[:4].tolist() == [0.0, 1.0, 0.0, 1.0] and torch.isnan(db[4])
+    x = torch.full((70, 5), 300.0, dtype=t, device="cuda")
+    w = torch.full((4, 5), -250.0, dtype=t, device="cuda")      # preactivation -375 000
+    y, kept = linear(x, w, activation=act, return_preactivation=True)
+    assert (y == 0).all() and (t != torch.float16 or torch.isinf(kept).all())
+    dx, dw, db = linear_backward(torch.ones_like(y), x, w, activation=act, preactivation=kept)
+    assert (dx == 0).all() and (dw == 0).all() and (db == 0).all()
