@@ -15,7 +15,8 @@
 // The backward's column sums are kept in registers over all rows that a wave walks, joined inside
 // the workgroup in LDS, written as one partial row per workgroup and joined by a second launch in
 // a fixed order, in double: no atomics, the same bits on every run.
-// All sums are in float (the join in double); the one rounding is that of the stored result.
+// All sums are in float (the join, and the longer chains of rows beyond 8192 elements, in double); the one
+// rounding is that of the stored result.
 // Measured: forward, 96 000 x 1280 float16, 96 us a call = 5.2 TB/s; backward, 48 000 x 1280 bfloat16, 72 us =
 // 5.1 TB/s, 5 of them the join (a 246 MB copy: 4.64 TB/s).  8 x 1280: 5 us, a call 13 with the host's work.
 #include "nn_common.h"
@@ -227,23 +228,24 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(ln::Args p) {
   }
 }
 
-// Rows longer than a workgroup's registers: one workgroup per row, the row read again for every sum.
+// Rows longer than a workgroup's registers: one workgroup per row, the row read again for every sum.  A
+// thread's chains, dim / 256 terms of up to 131 072, are in double.
 template <class T, class W>
 __global__ __launch_bounds__(256) void ln_fwd_long_kernel(ln::Args p) {
   using namespace ln;
   __shared__ float red[4], red2[4][2];
   const T* __restrict__ x = static_cast<const T*>(p.x) + (long long)blockIdx.x * p.x_stride;
   T* __restrict__ y = static_cast<T*>(p.out) + (long long)blockIdx.x * p.dim;
-  float s = 0.0f;
-  for (int i = threadIdx.x; i < p.dim; i += 256) s += (float)x[i];
-  const float mean = row_sum<256>(s, red) / p.fdim;
-  s = 0.0f;
-  float q = 0.0f;
+  double chain = 0.0, squares = 0.0;
+  for (int i = threadIdx.x; i < p.dim; i += 256) chain += (double)x[i];
+  const float mean = row_sum<256>((float)chain, red) / p.fdim;
+  chain = 0.0;
   for (int i = threadIdx.x; i < p.dim; i += 256) {
-    const float d = (float)x[i] - mean;
-    s += d;
-    q = fmaf(d, d, q);
+    const double d = (double)((float)x[i] - mean);
+    chain += d;
+    squares = fma(d, d, squares);
   }
+  float s = (float)chain, q = (float)squares;
   row_sums<256>(s, q, red2);
   const float left = s / p.fdim, rstd = inverse_spread(left, q / p.fdim, p.eps);
   for (int i = threadIdx.x; i < p.dim; i += 256) {
@@ -264,33 +266,34 @@ __global__ __launch_bounds__(256) void ln_bwd_long_kernel(ln::Args p) {
   const T* __restrict__ dy = static_cast<const T*>(p.dy) + (long long)blockIdx.x * p.dy_stride;
   T* __restrict__ dx = static_cast<T*>(p.out) + (long long)blockIdx.x * p.dim;
   const float mean = p.mean[blockIdx.x], rstd = p.rstd[blockIdx.x];
-  float s1 = 0.0f, s2 = 0.0f;
+  double chain1 = 0.0, chain2 = 0.0;
   for (int i = threadIdx.x; i < p.dim; i += 256) {
     const float g = (float)dy[i] * (p.w ? (float)static_cast<const W*>(p.w)[i] : 1.0f);
-    s1 += g;
-    s2 = fmaf(g, ((float)x[i] - mean) * rstd, s2);
+    chain1 += (double)g;
+    chain2 = fma((double)g, (double)(((float)x[i] - mean) * rstd), chain2);
   }
-  s1 = row_sum<256>(s1, red) / p.fdim;
-  s2 = row_sum<256>(s2, red) / p.fdim;
+  const float s1 = row_sum<256>((float)chain1, red) / p.fdim;
+  const float s2 = row_sum<256>((float)chain2, red) / p.fdim;
   for (int i = threadIdx.x; i < p.dim; i += 256) {
     const float g = (float)dy[i] * (p.w ? (float)static_cast<const W*>(p.w)[i] : 1.0f);
     dx[i] = (T)(rstd * (g - s1 - ((float)x[i] - mean) * rstd * s2));
   }
 }
-// column sums of the long rows: workgroup (x, y) adds rows y, y + gridDim.y, ... of 256 columns
+// column sums of the long rows: workgroup (x, y) adds rows y, y + gridDim.y, ... of 256 columns (up to 2^18 of
+// them in one chain: in double)
 template <class T>
 __global__ __launch_bounds__(256) void ln_columns_kernel(ln::Args p) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= p.dim) return;
-  float dw = 0.0f, db = 0.0f;
+  double dw = 0.0, db = 0.0;
   for (long long row = blockIdx.y; row < p.rows; row += gridDim.y) {
     const float g = (float)static_cast<const T*>(p.dy)[row * p.dy_stride + i];
     const float h = ((float)static_cast<const T*>(p.x)[row * p.x_stride + i] - p.mean[row]) * p.rstd[row];
-    dw = fmaf(g, h, dw);
-    db += g;
+    dw = fma((double)g, (double)h, dw);
+    db += (double)g;
   }
-  p.partial[((long long)blockIdx.y * 2) * p.dim + i] = dw;
-  p.partial[((long long)blockIdx.y * 2 + 1) * p.dim + i] = db;
+  p.partial[((long long)blockIdx.y * 2) * p.dim + i] = (float)dw;
+  p.partial[((long long)blockIdx.y * 2 + 1) * p.dim + i] = (float)db;
 }
 
 // out[i] = sum over groups of partial[group][i], i < n, in a fixed order: 32 columns per workgroup, each
