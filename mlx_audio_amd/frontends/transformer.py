@@ -9,8 +9,9 @@ anything else is copied first.  Host arrays are moved to the GPU.  Work is enque
 stream; nothing synchronises, so all functions can be captured into a graph.
 
 These functions record no autograd graph: the gradients come from the `*_backward` functions.
-Inputs that require a gradient are refused while gradients are enabled, so that none is lost
-silently (wrap the calls in `torch.no_grad()`).
+Inputs that require a gradient are refused while gradients are enabled (wrap the calls in
+`torch.no_grad()`), and so are inputs that carry a tangent of forward-mode differentiation: neither
+is lost silently.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._runtime import require_gpu
@@ -32,6 +34,7 @@ _ACTIVATIONS = {None: _lib.ACT_NONE, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.AC
 def _operands(**given) -> dict:
     """The given arrays as tensors of a supported type that need no gradient, without the absent ones."""
     out = {}
+    duals = getattr(forward_ad, "_current_level", 0) >= 0  # (inside a level; asking each tensor takes a microsecond)
     for name, x in given.items():
         if x is None:
             continue
@@ -42,6 +45,9 @@ def _operands(**given) -> dict:
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient, which this function does not record: call the "
                                "*_backward function for it, under torch.no_grad()")
+        if duals and forward_ad.unpack_dual(x).tangent is not None:
+            raise RuntimeError(f"{name} carries a tangent, which this function does not propagate: pass "
+                               "torch.autograd.forward_ad.unpack_dual(x).primal")
         out[name] = x
     return out
 
