@@ -48,6 +48,8 @@ def _operands(**given) -> dict:
         if duals and forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError(f"{name} carries a tangent, which this function does not propagate: pass "
                                "torch.autograd.forward_ad.unpack_dual(x).primal")
+        if x.is_neg():  # (a view with its sign pending, as of a conjugate's imaginary part)
+            x = x.resolve_neg()
         out[name] = x
     return out
 

@@ -6,6 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 from mlx_audio_amd import _lib, frontends as f
+from mlx_audio_amd.frontends import transformer
 
 
 @pytest.mark.parametrize("sizes", [(0, 5, 7), (1, 0, 7), (1, 5, 0), (0, 0, 0), (3, 1, 1), (2, 1500, 1500)])
@@ -40,3 +41,13 @@ def test_a_tangent_is_never_lost_silently():
             for call in calls(torch.randn(4, 8)) + calls(forward_ad.unpack_dual(x).primal):
                 with pytest.raises(RuntimeError, match="no CPU fallback"):
                     call()
+
+
+def test_negated_views_are_taken_as_what_they_mean():
+    """The imaginary part of a conjugate is a view of the stored values with the sign pending."""
+    z = torch.randn(6, 1, dtype=torch.complex64)
+    view = z.conj().imag
+    assert view.is_neg() and view.stride(-1) != 0
+    got = transformer._operands(x=view, weight=view[0])
+    assert not any(t.is_neg() for t in got.values())
+    assert torch.equal(got["x"], -z.imag) and torch.equal(got["weight"], -z.imag[0])
