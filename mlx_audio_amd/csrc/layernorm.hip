@@ -19,7 +19,7 @@
 // rounding is that of the stored result.
 // Measured: forward, 96 000 x 1280 float16, 96 us a call = 5.2 TB/s; backward, 48 000 x 1280 bfloat16, 72 us =
 // 5.1 TB/s, 5 of them the join (a 246 MB copy: 4.64 TB/s).  8 x 1280: 5 us, a call 13 with the host's work.
-#include "nn_common.h"
+#include "column_sums.h"
 
 namespace mia {
 namespace ln {
@@ -296,34 +296,6 @@ __global__ __launch_bounds__(256) void ln_columns_kernel(ln::Args p) {
   p.partial[((long long)blockIdx.y * 2 + 1) * p.dim + i] = (float)db;
 }
 
-// out[i] = sum over groups of partial[group][i], i < n, in a fixed order: 32 columns per workgroup, each
-// of its 32 slices every 32nd group.
-__global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__ partial, int groups, int n,
-                                                       float* __restrict__ dw, float* __restrict__ db, int dim) {
-  __shared__ double part[32][32];
-  const int slice = threadIdx.x >> 5, c = threadIdx.x & 31;
-  const int i = blockIdx.x * 32 + c;
-  double s[2] = {};
-  if (i < n) {
-    int g = slice;
-    for (; g + 96 < groups; g += 128) {  // four loads in flight
-      const float a = partial[(long long)g * n + i], b = partial[(long long)(g + 32) * n + i];
-      const float d = partial[(long long)(g + 64) * n + i], e = partial[(long long)(g + 96) * n + i];
-      s[0] += (double)a + (double)b;
-      s[1] += (double)d + (double)e;
-    }
-    for (; g < groups; g += 32) s[0] += (double)partial[(long long)g * n + i];
-  }
-  part[slice][c] = s[0] + s[1];
-  __syncthreads();
-  if (slice == 0 && i < n) {
-    double t = 0.0;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) t += part[k][c];
-    (i < dim ? dw[i] : db[i - dim]) = (float)t;
-  }
-}
-
 namespace ln {
 constexpr int kMaxGroups = 512;   // workgroups of the backward: two per compute unit
 constexpr int kLongGroups = 64;   // row groups of the long rows' column sums
@@ -467,7 +439,7 @@ int mia_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
   }
   if (dweight) {
     const int n = (int)(2 * dim);
-    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s,
+    hipLaunchKernelGGL(nn::join_columns_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s,
                        static_cast<const float*>(workspace), groups, n, dweight, dbias, (int)dim);
   }
   MIA_CHECK_HIP(hipGetLastError());

@@ -1,35 +1,8 @@
 // C entry points of the linear layer (kernels: linear_kernels.h, one translation unit per element type).
+#include "column_sums.h"
 #include "linear_kernels.h"
 
 namespace mia {
-// out[i] = sum of the groups' partial sums in a fixed order, in double: 32 columns per workgroup, each of
-// its 32 slices every 32nd group
-__global__ __launch_bounds__(1024) void lin_bias_join_kernel(const float* __restrict__ partial, int groups, int n,
-                                                            float* __restrict__ out) {
-  __shared__ double part[32][32];
-  const int slice = threadIdx.x >> 5, c = threadIdx.x & 31;
-  const int i = blockIdx.x * 32 + c;
-  double s[2] = {};
-  if (i < n) {
-    int g = slice;
-    for (; g + 96 < groups; g += 128) {  // four loads in flight
-      const float a = partial[(long long)g * n + i], b = partial[(long long)(g + 32) * n + i];
-      const float d = partial[(long long)(g + 64) * n + i], e = partial[(long long)(g + 96) * n + i];
-      s[0] += (double)a + (double)b;
-      s[1] += (double)d + (double)e;
-    }
-    for (; g < groups; g += 32) s[0] += (double)partial[(long long)g * n + i];
-  }
-  part[slice][c] = s[0] + s[1];
-  __syncthreads();
-  if (slice == 0 && i < n) {
-    double t = 0.0;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) t += part[k][c];
-    out[i] = (float)t;
-  }
-}
-
 namespace lin {
 constexpr long long kMaxSize = (1LL << 30) - 4096;  // positions along k are counted in 32 bits
 constexpr long long kMaxWidth = 1LL << 26;          // and so are a launch's threads (up to 32 a column)
@@ -131,8 +104,8 @@ int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_
       if (dz) g = dz, g_stride = out;
     }
     if (dbias) {
-      hipLaunchKernelGGL(lin_bias_join_kernel, dim3((unsigned)((out + 31) / 32)), dim3(1024), 0, s, sums, groups,
-                         (int)out, dbias);
+      hipLaunchKernelGGL(nn::join_columns_kernel, dim3((unsigned)((out + 31) / 32)), dim3(1024), 0, s, sums, groups,
+                         (int)out, dbias, static_cast<float*>(nullptr), (int)out);
     }
     lin::Epilogue e{nullptr, 0, MIA_ACT_NONE, nullptr, 0, nullptr, nullptr};
     if (dx && rows) {

@@ -158,8 +158,8 @@ __device__ __forceinline__ u4 load_residual(const Epilogue& e, long long m, int 
   return load_piece(static_cast<const T*>(e.residual) + m * e.residual_stride + n, left);
 }
 
-// 64 bytes that read as zero: the source of every piece that lies outside its operand.
-__device__ const u4 kZeros[4] = {};
+// reads as zero: the source of every piece that lies outside its operand
+__device__ const u4 kZeros[1] = {};
 }  // namespace lin
 
 // Tile of BN x BM results, WN x WM waves.  An LDS stage holds 128 bytes of k (two matrix steps) of both
