@@ -73,14 +73,16 @@ struct Shape {
   static constexpr int PW = BYTES / 4096;          // 1 KiB pieces per wave and tile
 };
 
-// Piece c of LDS row r lies at position c ^ turn(r), so that neither kind of read meets itself on a
-// bank: one piece of 16 rows (turn differs for rows that start on the same banks), or 32 bytes of
-// each of 8 rows down the columns (turn / 2 differs too; float: 64 bytes of every fourth row, turn / 4).
+// Piece c of LDS row r lies at position c ^ turn(r), so that neither kind of read meets itself on one of the
+// 64 banks.  Reads of 16 bytes are served 16 lanes at a time, lanes 0-3, 12-15, 20-23, 24-27, then 4-7, 8-11,
+// 16-19, 28-31, and so on: rows 0-3 and 12-15 of piece g with rows 4-11 of piece g + 1, which lie apart because
+// turn is even (a turn by bit 3 of the row as well brought them together: 4 cycles more for each such read, 33 -
+// 40 % of all LDS cycles; without it the counter says none).  Reads down the columns are served 32 lanes at a
+// time: 32 bytes of each of 8 rows, whose turn / 2 differs (float: 64 bytes of every fourth row, turn / 4).
 template <class T, int DP>
 __device__ __forceinline__ int turn(int r) {
   if (sizeof(T) == 4) return r & 15;
-  if (DP <= 64) return (r & 6) | ((r >> 3) & 1);
-  return ((r & 7) << 1) | ((r >> 3) & 1);
+  return DP <= 64 ? r & 6 : (r & 7) << 1;
 }
 // A lane's place in LDS for either kind of read of a tile that starts at byte `tile` (a multiple of 1024),
 // worked out once: every other address is it, with bits above the bank turned (^) and constants added.
