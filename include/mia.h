@@ -610,7 +610,7 @@ int mia_linear(const void* x, int64_t x_stride, const void* weight, int64_t weig
 /* The gradients with dz = dy act'(preactivation): dx = dz weight (rows, in), dweight = dz^T x
  * (out, in), both contiguous of the operands' type, dbias = sum over rows of dz, float32 (out); each
  * may be NULL.  The residual's gradient is dy itself.  dz is rounded to the operands' type for the
- * two products (the matrix cores take no other), not for dbias. */
+ * two products (the matrix cores take no other; float16: to multiples of 2^-24, as dy is), not for dbias. */
 size_t mia_linear_backward_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype, int activation);
 int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* weight,
                         int64_t weight_stride, const void* preactivation, int64_t preactivation_stride, int activation,
@@ -625,6 +625,7 @@ int mia_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_
  * contiguous [batch, queries, heads, dim] of q's type; lse: float32 (batch, heads, queries), the
  * logarithm of the sum of exponentials, or NULL (the backward pass needs it).  A value that is not
  * finite in a key or value row that SOME query of a causal call sees may reach other queries.
+ * Two-byte types: the probabilities are rounded to the type for the product with v (up to 64 queries: in two parts).
  * A call may have fewer than 2^24 workgroups of 64 or 128 rows (of each batch item and head, parts
  * of a split included): MIA_ERR_UNSUPPORTED beyond, before anything is enqueued.
  * workspace: mia_attention_workspace_bytes bytes, 16-byte aligned (0 unless the keys are split). */
@@ -642,7 +643,9 @@ int mia_attention(const mia_attention_desc* desc, const void* q, const void* k, 
                   void* stream);
 /* The gradients, with the probabilities recomputed from lse: dq [batch, queries, heads, dim], dk and
  * dv [batch, keys, kv_heads, dim] (summed over the query heads that share a key head; zero behind a
- * length), contiguous.  out and lse are what the forward call wrote; dout and out by strides. */
+ * length, whatever dout holds), contiguous.  out and lse are what the forward call wrote; dout and out by
+ * strides.  Two-byte types: probabilities and their gradients are rounded to the type for the products (dq with up
+ * to 64 queries: in two parts), in float16 times powers of two that keep them from its limits at either end. */
 size_t mia_attention_backward_workspace_bytes(const mia_attention_desc* desc);
 int mia_attention_backward(const mia_attention_desc* desc, const void* dout, const int64_t* stride_dout,
                            const void* q, const void* k, const void* v, const void* out, const int64_t* stride_out,

@@ -131,7 +131,8 @@ __device__ __forceinline__ u4 columns_fragment(unsigned place, int st, int dt) {
     return x;
   }
 }
-// the product tiles of one step as the next product's second operand
+// the product tiles of one step as the next product's second operand.  Two-byte types are rounded here, the type
+// that the matrix instruction takes: one rounding beside the stored result's, 1.4 of it together.
 template <class T>
 __device__ __forceinline__ u4 to_operand(const f4* blocks) {
   if constexpr (sizeof(T) == 2) {
@@ -370,9 +371,10 @@ __device__ __forceinline__ void scale_own(u4 (&v)[N], int e) {
 }
 }  // namespace att
 
-// Forward.  OT: blocks of 16 queries per wave.  bfloat16, 8 x 1500, 20 heads of 64: 139 us (663 TFLOP/s), bound by the
-// vector ALUs: 209 instructions beside 32 matrix ones for 64 keys x 32 queries.  Four waves per SIMD (128 registers)
-// instead of three: 157 -> 140.  4 x 2048, 16 heads of 128: 148 us (927).  One query on 1500 keys, 16 items, 20 heads:
+// Forward.  OT: blocks of 16 queries per wave.  bfloat16, 8 x 1500, 20 heads of 64: 118 - 125 us (740 - 780 TFLOP/s),
+// of which the vector ALUs are busy 89: for 64 keys x 32 queries 175 instructions and 32
+// exponentials beside 32 matrix ones (38 us); the rest of the time the four waves of a SIMD do not overlap.  Four waves
+// (128 registers) instead of three: 157 -> 140.  4 x 2048, 16 heads of 128: 148 us (927).  One query on 1500 keys, 16 items, 20 heads:
 // 26 us with the join, HBM.
 // BOTH: what the rounding of p to a two-byte type takes away goes through a second product, and the error falls from
 // 1.39 to 1.00 of a result rounded once.  For calls whose rows (up to 64 of a pair) fit one workgroup: memory sets
@@ -834,7 +836,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(att::Args p) {
 }
 
 // dk and dv: own rows are keys, q and dout stream, over all heads that share the key head.  With dq, bfloat16,
-// 8 x 1500, 20 heads of 64: 410 us.  Two waves per SIMD: for three the registers spill (438 -> 552 us).
+// 8 x 1500, 20 heads of 64: 359 us.  Two waves per SIMD: for three the registers spill (438 -> 552 us).
 template <class T, int DP, int OT, bool DMA>
 __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void att_dkv_kernel(att::Args p) {
   using namespace att;

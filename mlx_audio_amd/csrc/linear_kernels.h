@@ -183,8 +183,9 @@ using LinTile64 = LinTile<64, 64, 1, 4, 4>;
 namespace lin {
 // One operand's tile in LDS and its fragments.  KC: k contiguous, LDS rows are `ROWS` operand rows
 // of eight 16-byte pieces of k; otherwise LDS rows are the stage's k, ROWS elements each.  Piece c of
-// LDS row r sits at piece position c ^ swizzle(r), so that the lanes of one LDS read fall on
-// different banks; with LDS-DMA the same permutation is applied to the source addresses.
+// LDS row r sits at piece position c ^ swizzle(r), so that the lanes served together by an LDS read fall on
+// different banks (the counter of the forward product says no conflicts), but for column reads with Q = 8,
+// below; with LDS-DMA the same permutation is applied to the source addresses.
 template <class T, bool KC, int ROWS, int Q>
 struct Operand {
   static constexpr int ES = (int)sizeof(T), V = 16 / ES;
@@ -210,8 +211,9 @@ struct Operand {
   // The 16-byte fragment of tile row row0 + Q (r >> 2) + (r & 3), r = lane & 15, k piece 4 sub + (lane >> 4).
   // Q = 4: rows in order.  Q = 8 (two-byte types, first operand): the accumulators at row0 = base and
   // base + 4 together give lane group g of the result the rows base + 8 g ... + 7, so that a store of
-  // 16 bytes a lane writes 64 consecutive bytes of 16 rows.  (Down the columns Q = 8 uses half of the
-  // LDS banks at a time; with Q = 4 and stores of 8 bytes the gradients took 2 - 8 % longer.)
+  // 16 bytes a lane writes 64 consecutive bytes of 16 rows.  (Down the columns Q = 8 takes 8 of
+  // every 16 bytes, half of the LDS banks, and each read twice its cycles: 40 % of the LDS cycles in dx, 33 % in
+  // dW are such conflicts; with Q = 4 and stores of 8 bytes the gradients took 2 - 9 % longer.)
   static __device__ __forceinline__ u4 fragment(const unsigned char* tile, int row0, int sub, int lane) {
     const int r15 = lane & 15, g = lane >> 4;
     if constexpr (KC) {
@@ -577,7 +579,7 @@ __global__ __launch_bounds__(TL::WG, TL::OCC) void lin_gemm_kernel(lin::Gemm p) 
 // a tile the results are stored while the next tile's first stages arrive; a wave waits for its loads,
 // never for the stores behind them (loads and stores are counted in order: "all but the newest STORES").
 // Measured, bfloat16: 8192^3 802 us (1 372 TFLOP/s); 24000 x 1280 -> 5120 351 us (897; with GELU and the
-// preactivation 388), 24000 x 5120 -> 1280 259 (1 214).  A stage takes 1.57 us, of which the matrix instructions
+// preactivation 389 - 396), 24000 x 5120 -> 1280 259 (1 214).  A stage takes 1.57 us, of which the matrix instructions
 // need 0.85 at 2.4 GHz; reading fragments and multiplying share the rest.  Short k is bound by the tile's end.
 template <class TL, class T, bool AKC, bool BKC>
 __global__ __launch_bounds__(TL::WG, 1) void lin_gemm8_kernel(lin::Gemm p) {
@@ -738,7 +740,7 @@ __global__ __launch_bounds__(64 * NW) void lin_few_kernel(lin::Gemm p) {
 }
 
 // dz = dy act'(z), rounded to the operands' type for the two products that read it, and the column
-// sums of the unrounded values: workgroup (x, y) takes rows y, y + gridDim.y ... of 64 pieces of 16
+// sums of the unrounded values (float16: dz is a multiple of 2^-24, as dy is): workgroup (x, y) takes rows y, y + gridDim.y ... of 64 pieces of 16
 // bytes, four rows at a time (one per wave).  24000 x 5120, bfloat16: 150 us, 4.9 TB/s.
 // z null: no activation, sums only (dz null too).
 template <class T>

@@ -5,8 +5,9 @@ pass (the blocks `AudioEncoder.__call__` runs after the stem, models/whisper/lay
 Element types are float32, float16 and bfloat16; every sum, statistic and intermediate value is
 float32, and results are rounded once.  Tensors may be views: rows (the last axis) must be
 contiguous and the leading axes of `layer_norm` / `linear` inputs collapse to rows of one stride,
-anything else is copied first.  Host arrays are moved to the GPU.  Work is enqueued on the current
-stream; nothing synchronises, so all functions can be captured into a graph.
+anything else is copied first.  Host arrays (lists of key_lengths among them) are moved to the GPU by
+a copy that waits.  With operands on the device nothing synchronises: work is enqueued on the current
+stream and can be captured into a graph.
 
 These functions record no autograd graph: the gradients come from the `*_backward` functions.
 Inputs that require a gradient are refused while gradients are enabled (wrap the calls in
@@ -242,7 +243,8 @@ def linear_backward(dy, x, weight, activation=None, preactivation=None, input_gr
     dy [..., out], x [..., in], weight [out, in] and preactivation [..., out] (what the forward call
     returned; needed for an activation) of one type.  dx and dweight have that type, dbias is
     float32; a gradient not asked for is None.  The residual's gradient is dy itself.  For the two
-    products dz is rounded to the operands' type.
+    products dz is rounded to the operands' type: in float16 to multiples of 2^-24 at the finest, as
+    dy itself is, so a dy below 1e-4 wants a scaled loss.
     """
     ops = _operands(dy=dy, x=x, weight=weight, preactivation=preactivation)
     dy, x, weight, z = ops["dy"], ops["x"], ops["weight"], ops.get("preactivation")
@@ -339,8 +341,9 @@ def attention(q, k, v, causal: bool = False, key_lengths=None, scale=None, retur
     Returns out [B, Sq, H, D], contiguous; with return_lse also the logarithm of each row's sum of
     exponentials, float32 [B, H, Sq] (-inf where no key is seen), which `attention_backward` takes.
     Few queries over many keys (a decoding step) are split along the keys and joined.  The
-    probabilities of two-byte types are rounded to that type for the product with v, except with at
-    most 64 queries: those lose nothing.
+    probabilities of two-byte types are rounded to that type for the product with v (relative eps / 2;
+    float16 at least 2^-25 of a row's largest), except with at most 64 queries: those go in as the
+    rounded value and the rest, itself rounded (eps / 2 squared, and the same 2^-25).
     """
     ops = _operands(q=q, k=k, v=v)
     _same_type(ops, ("q", "k", "v"))
