@@ -150,3 +150,58 @@ def test_lengths_views_and_shared_heads(gpu, dim):
     want = exact(dout[1:2], q[1:2], k[1:2, :37], v[1:2, :37], out[1:2], lse[1:2])
     assert max(against_one_rounding(g[1:2, :n], w) for g, w, n in zip(got, want, (150, 37, 37))) <= 1.5
     assert all((g[1, 37:] == 0).all() and (g[2] == 0).all() for g in got[1:]) and (got[0][2] == 0).all()
+
+
+def test_no_items_queries_or_keys(gpu):
+    for B, Sq, Sk in ((0, 5, 7), (2, 0, 7), (2, 5, 0), (0, 0, 0)):
+        q, kv = make((B, Sq, 4, 40), HALF, 40), make((B, Sk, 2, 40), HALF, 41)
+        out, lse = attention(q, kv, kv, return_lse=True)
+        dq, dk, dv = attention_backward(q, q, kv, kv, out, lse)
+        assert dq.shape == q.shape and dk.shape == dv.shape == kv.shape
+        assert all((g == 0).all() for g in (dq, dk, dv))
+
+
+def test_one_gradient_for_every_query(gpu):
+    """dout expanded along items, queries and heads (the gradient of a sum), against its copy."""
+    q, k, v = make((3, 70, 4, 64), HALF, 42), make((3, 90, 2, 64), HALF, 43), make((3, 90, 2, 64), HALF, 44)
+    dout = make((64,), HALF, 45, 1e-3).expand(3, 70, 4, 64)
+    out, lse = attention(q, k, v, return_lse=True)
+    got, want = attention_backward(dout, q, k, v, out, lse), attention_backward(dout.contiguous(), q, k, v, out, lse)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    assert max(against_one_rounding(g, w) for g, w in zip(got, exact(dout, q, k, v, out, lse))) <= 1.5
+
+
+def test_many_items_and_many_heads_on_one_key_head(gpu):
+    q, k, v = make((300, 9, 8, 32), HALF, 46), make((300, 20, 1, 32), HALF, 47), make((300, 20, 1, 32), HALF, 48)
+    dout = make(q.shape, HALF, 49, 1e-4)
+    lengths = [(7 * i) % 21 for i in range(300)]
+    out, lse = attention(q, k, v, key_lengths=lengths, return_lse=True)
+    got = attention_backward(dout, q, k, v, out, lse, key_lengths=lengths)
+    for b in (0, 1, 2, 150, 299):
+        n = lengths[b]
+        want = exact(dout[b:b + 1], q[b:b + 1], k[b:b + 1, :n], v[b:b + 1, :n], out[b:b + 1], lse[b:b + 1]) if n else None
+        if n:
+            alone = attention_backward(*(x[b:b + 1] for x in (dout, q)), k[b:b + 1, :n], v[b:b + 1, :n], out[b:b + 1], lse[b:b + 1])
+            assert torch.equal(got[0][b], alone[0][0])
+            assert max(against_one_rounding(g[b:b + 1, :m], w) for g, w, m in zip(got, want, (9, n, n))) <= 1.6  # (few values)
+        assert (got[1][b, n:] == 0).all() and (got[2][b, n:] == 0).all()
+
+
+def test_calls_at_once_on_two_streams(gpu):
+    sets = []
+    for i, size in enumerate((1.0, 1e-4)):
+        q, k, v = make((4, 300, 8, 64), HALF, 50 + i), make((4, 300, 8, 64), HALF, 52 + i), make((4, 300, 8, 64), HALF, 54 + i)
+        dout = make(q.shape, HALF, 56 + i, size)
+        out, lse = attention(q, k, v, return_lse=True)
+        sets.append((dout, q, k, v, out, lse))
+    want = [attention_backward(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(attention_backward(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, c) for one in got[i] for a, c in zip(one, want[i]))
