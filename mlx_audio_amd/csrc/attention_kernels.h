@@ -1172,7 +1172,7 @@ int Ops<T>::backward(Args a, float* stats, void* dq, void* dk, void* dv, hipStre
   if constexpr (std::is_same<T, _Float16>::value) {
     a.range = a.partial, a.range_parts = range_parts(a.batch, a.sq, a.sk, a.heads, a.kv_heads);
     a.partial += range_bytes(a.batch, a.kv_heads, a.range_parts) / sizeof(float);
-    const long long range_grid = (long long)a.batch * a.kv_heads * a.range_parts;  // (no more than dkv's, or 64 a pair)
+    const long long range_grid = (long long)a.batch * a.kv_heads * a.range_parts;
     const int fits = check_grid(range_grid);
     if (fits != MIA_OK) return fits;
     hipLaunchKernelGGL(att_range_kernel<T>, dim3((unsigned)range_grid), dim3(256), 0, s, a);
